@@ -136,6 +136,11 @@ int sh_file_block(const sh_file* f, const void** data, size_t* size);
 
 /* ---- engine: imi_seoul::load / reset / step / step2 / step_batch / new_state / swap_state ---- */
 int sh_create(int device, sh_ctx** out);
+/* The same on the caller's own stream (a hipStream_t of `device`; null: the device's default stream): everything the
+ * context enqueues runs in order with the caller's other work there, and a graph captured on that stream holds it. The
+ * stream must outlive the context, which does not destroy it. On the default stream, which cannot be captured, the
+ * engine's steps run without their graph (the same kernels, the same numbers). */
+int sh_create_on(int device, void* stream, sh_ctx** out);
 int sh_destroy(sh_ctx* ctx);
 /* Read a GGUF brain file, repack every Q4_0 table into the device layout and upload it; n_ctx = context length of
  * states made afterwards (imi/core/seoul.cpp:93-186). */
@@ -310,6 +315,89 @@ int sh_voice_feedback(sh_voice* v, const int32_t* codes, float* out);
  * n_vocab <= 4096, temp > 0, rep > 0. */
 int sh_voice_sample(sh_voice* v, const int32_t* hist, int n_frames, const double* u, float temp, float rep,
                     int32_t* picks, double* keep);
+
+/* ---- a batch of conversations: pages of keys and values, attention over them, the next words ----
+ * No counterpart in the reference, which holds one or two conversations, each in a cache of its own (imi/core/seoul.h:
+ * 21-26), and picks greedily (imi/core/hear.cpp:66-72). All pointers are device memory on the context's device; calls are
+ * enqueued on the context's stream without waiting (sh_sync waits), allocate nothing and may be captured into a graph.
+ * Lengths, tables and slots live on the device, so what they hold is checked there: an entry that points outside its
+ * array is treated as said below and never followed. Arrays of 16-bit types, keys and values start on 16 bytes.
+ *
+ * A cache is keys and values in pages of `page` positions, for one layer: [n_pages][n_kv][page][head_dim] each. A slot is
+ * a place for one position: page id * page + position in the page. Types as in sh_tensor: SH_F32, SH_F16, SH_BF16. */
+#define SH_F32 0
+#define SH_F16 1
+#define SH_BF16 30
+
+typedef struct {
+    int n_head, n_kv, head_dim;     /* n_head a multiple of n_kv; head_dim 32, 64 or 128 */
+    int page;                       /* positions per page: 16, 32, 64, 128 or 256 */
+    int type;                       /* keys, values, queries and outputs: SH_F16 or SH_BF16 */
+    int window;                     /* a position sees itself and the window - 1 before it; 0: everything before it */
+    long long n_pages;
+    float scale;                    /* of the scores; 0: 1 / sqrt(head_dim) */
+    float eps;                      /* of the head norms (sh_page_put) */
+} sh_page_shape;
+
+/* Block tables and slot maps of a step from the lengths of its requests. Request i holds held[i] positions in pages
+ * (table[i][0 .. ceil(held/page)), row stride `cols`) and gets add[i] more. Requests are served in order: the pages that
+ * request i needs besides its own are taken from free_pages[taken ...], where *taken counts those given out before.
+ *   table      [n][cols]  the new entries are written, the others stay
+ *   len        [n]        held + add; held where the request is refused
+ *   cu         [n + 1]    rows of the step before each request (running sum of add; a negative add counts as 0)
+ *   slots, pos [rows]     of each new row: its slot (-1: none) and its position, pos0 + held + its place among the new ones
+ *   taken_out  [1]        pages given out after the step
+ * A request is refused (slots -1, no pages) when a length is negative, its pages pass `cols`, its rows pass `rows`, or
+ * free_pages has not enough left for it and those before it. Entries of slots and pos behind the last request's rows stay
+ * as they were. n up to 4096. No output may overlap an input (SH_E_ARG). */
+int sh_page_plan(sh_ctx* ctx, int n, const int32_t* held, const int32_t* add, int page, int32_t* table, int cols,
+                 const int32_t* free_pages, int n_free, const int32_t* taken, int32_t* taken_out, int32_t* len,
+                 int32_t* cu, int64_t* slots, int32_t* pos, int rows, int pos0);
+
+/* Queries, keys and values of `rows` positions out of packed rows qkv [rows][ld] (q heads, k heads, v heads, whatever
+ * else; src_type SH_F32, SH_F16 or SH_BF16), as the packed attention table gives them: RMS norm over each q and k head
+ * (q_norm, k_norm [head_dim]; null: none), rotation of the pairs (i, i + head_dim / 2) by rope[pos][i] = (cos, sin)
+ * (null: none; n_rope positions), one rounding to the shape's type, keys and values to their slots, queries to
+ * q_out [rows][n_head][head_dim] (null: none). A row whose slot is negative or past the cache writes no keys and values;
+ * one whose position is outside the rotation table writes none either, and zeros for its queries. No two rows may have
+ * the same slot. The reference does this per position (imi/core/seoul.cpp:19-28, 407-431). */
+int sh_page_put(sh_ctx* ctx, const sh_page_shape* shape, int rows, const void* qkv, long long ld, int src_type,
+                const float* q_norm, const float* k_norm, const float* rope, int n_rope, const int32_t* pos,
+                const int64_t* slots, void* q_out, void* keys, void* values);
+
+/* Attention of a batch whose requests share their first prefix_len positions (pages prefix[0 .. ceil(prefix_len/page));
+ * 0: nothing shared) and have own ones behind them: request i holds len[i] (at most max_len) positions in the pages
+ * table[i] (row stride cols). Its query rows are cu[i] .. cu[i + 1] - 1 (at most max_rows), its last positions in order; cu null: one
+ * row for each request, rows == n. Row r sees the shared positions, its request's own up to its own position, and of
+ * these the shape's window. out[r][h] = sum of softmax(scale q k) v, times sigmoid(gate[r][h]) where gate [rows][n_head]
+ * is given (imi/core/seoul.cpp:433-453); lse [rows][n_head] (null: none) gets the logarithm of the sum of e^score, before
+ * the gate. A row that sees nothing gives zeros and -inf. Keys of a page id outside [0, n_pages) count as not there. Rows
+ * behind the last request's, and those past max_rows of their request, stay as they were.
+ * The shared positions are read once for the whole batch, as one matrix product for all rows. work: sh_page_attn_work's
+ * bytes for the same sizes, on 256 bytes, the call's own until it is done (calls that may run at once, captured graphs
+ * among them, need one each; nothing is kept in it between calls). */
+int sh_page_attn_work(const sh_page_shape* shape, int n, int rows, int max_rows, int prefix_len, int max_len,
+                      size_t* bytes);
+int sh_page_attn(sh_ctx* ctx, const sh_page_shape* shape, int n, int rows, const int32_t* cu, int max_rows, const void* q,
+                 const void* keys, const void* values, const int32_t* prefix, int prefix_len, const int32_t* table,
+                 int cols, const int32_t* len, int max_len, const float* gate, void* out, float* lse, void* work,
+                 size_t work_bytes);
+
+/* One word for each row of scores [rows][vocab] (type SH_F32, SH_F16 or SH_BF16; row stride ld): with weights
+ * e^((score - max) / temp), words in the order of their scores (equal ones by index), kept are
+ *   the first top_k (<= 0: all), of these the shortest beginning whose weights reach top_p of their sum (>= 1: all,
+ *   at least one word), of these the weights of at least min_p times the largest (<= 0: all);
+ * ids[row] = the first kept index at which the sum of the kept weights in index order exceeds u[row] times their sum
+ * (u in [0, 1): the caller's random numbers; below 0 counts as 0, from 1 on the last kept word is taken), chance[row]
+ * (null: none) = its weight over that sum. temp 0 takes the first index of the maximum, chance 1. Each of temp, top_k,
+ * top_p, min_p is one value per row or null (1, 0, 1, 0). Scores of -inf or NaN are never taken; a score of +inf leaves
+ * only those. A row with nothing to take, or whose temp is negative or NaN, gives -1 and chance 0. A NaN in u, top_p or
+ * min_p counts as 0, 1, 0. Weights are summed in 2^-44ths of the largest (smaller ones are never taken), vocab is at most
+ * 524288. sh_generate picks greedily, sh_voice_sample samples codes. work: sh_sample_work's bytes, as above. */
+int sh_sample_work(int rows, int vocab, size_t* bytes);
+int sh_sample(sh_ctx* ctx, int rows, int vocab, const void* scores, long long ld, int type, const float* temp,
+              const int32_t* top_k, const float* top_p, const float* min_p, const double* u, int32_t* ids, float* chance,
+              void* work, size_t work_bytes);
 
 /* Synchronise the context's stream (for callers of the _dev entry points). */
 int sh_sync(sh_ctx* ctx);

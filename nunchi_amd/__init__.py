@@ -19,7 +19,7 @@ LIB_PATH = os.path.join(HERE, "libseoul_hip.so")
 
 SH_OK, SH_E_ARG, SH_E_HIP, SH_E_FILE, SH_E_SHAPE, SH_E_CONTEXT_FULL, SH_E_STATE, SH_E_NOMEM = 0, -1, -2, -3, -4, -5, -6, -7
 EXPORTS = [
-    "sh_last_error", "sh_create", "sh_destroy", "sh_load", "sh_info", "sh_check_model", "sh_state_new", "sh_state_free", "sh_state_reset",
+    "sh_last_error", "sh_create", "sh_create_on", "sh_destroy", "sh_load", "sh_info", "sh_check_model", "sh_state_new", "sh_state_free", "sh_state_reset",
     "sh_state_pos", "sh_state_set_pos", "sh_step", "sh_step2", "sh_step_batch", "sh_generate", "sh_bench_tables",
     "sh_bench_kernel", "sh_bench_step_kernel",
     "sh_q4_create", "sh_q4_free", "sh_q4_rows", "sh_q4_gemv", "sh_q4_gemm", "sh_q4_gemm_noalloc", "sh_q4_gemv_dev", "sh_q4_bench", "sh_q4_bench_kernel", "sh_q4_bench_graph",
@@ -31,6 +31,7 @@ EXPORTS = [
     "sh_codec_load", "sh_codec_free", "sh_codec_info", "sh_codec_reset", "sh_codec_frame", "sh_codec_flush",
     "sh_ears_load", "sh_ears_free", "sh_ears_info", "sh_ears_positions", "sh_ears_encode", "sh_ears_mel",
     "sh_bench_empty", "sh_bench_read", "sh_bench_xcc", "sh_bench_l2_reuse",
+    "sh_page_plan", "sh_page_put", "sh_page_attn_work", "sh_page_attn", "sh_sample_work", "sh_sample",
 ]
 
 
@@ -86,6 +87,7 @@ def load_library(path: str = LIB_PATH):
     sig = {
         "sh_last_error": (C.c_char_p, []),
         "sh_create": (i, [i, P(vp)]),
+        "sh_create_on": (i, [i, vp, P(vp)]),
         "sh_destroy": (i, [vp]),
         "sh_load": (i, [vp, C.c_char_p, i]),
         "sh_info": (i, [vp, P(ModelInfo)]),
@@ -152,6 +154,12 @@ def load_library(path: str = LIB_PATH):
         "sh_ears_positions": (i, [vp, i, P(i), P(i)]),
         "sh_ears_encode": (i, [vp, vp, i, vp, P(i)]),
         "sh_ears_mel": (i, [vp, vp, i, P(i)]),
+        "sh_page_plan": (i, [vp, i, vp, vp, i, vp, i, vp, i, vp, vp, vp, vp, vp, vp, i, i]),
+        "sh_page_put": (i, [vp, vp, i, vp, C.c_longlong, i, vp, vp, vp, i, vp, vp, vp, vp, vp]),
+        "sh_page_attn_work": (i, [vp, i, i, i, i, i, P(C.c_size_t)]),
+        "sh_page_attn": (i, [vp, vp, i, i, vp, i, vp, vp, vp, vp, i, vp, i, vp, i, vp, vp, vp, vp, C.c_size_t]),
+        "sh_sample_work": (i, [i, i, P(C.c_size_t)]),
+        "sh_sample": (i, [vp, i, i, vp, C.c_longlong, i, vp, vp, vp, vp, vp, vp, vp, vp, C.c_size_t]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -252,13 +260,15 @@ _live_contexts = weakref.WeakSet()
 
 class Context:
     """One device and its stream (sh_create). States and tables made on it are freed before it is destroyed (the
-    C ABI requires it), whatever order the garbage collector finalizes them in."""
+    C ABI requires it), whatever order the garbage collector finalizes them in. With stream (a HIP stream's address,
+    0 for the default stream) the context enqueues on that stream of the caller's, which must outlive it."""
 
-    def __init__(self, device: int = 0):
+    def __init__(self, device: int = 0, stream: int | None = None):
         load_library()
         self.h = C.c_void_p()
+        self.device = int(device)
         self._children = weakref.WeakSet()
-        _check(_lib.sh_create(device, C.byref(self.h)))
+        _check(_lib.sh_create(device, C.byref(self.h)) if stream is None else _lib.sh_create_on(device, stream, C.byref(self.h)))
         _live_contexts.add(self)
 
     def _adopt(self, obj):
@@ -703,6 +713,9 @@ class Voice:
         _check(_lib.sh_voice_sample(self.h, _p(hist), hist.shape[0], _p(u), float(temp), float(rep), _p(picks),
                                     _p(keep)))
         return picks[:u.size], keep[:u.size]
+
+
+from .batch import (PageShape, page_attn, page_attn_work, page_plan, page_put, sample, sample_work)  # noqa: E402
 
 
 @atexit.register

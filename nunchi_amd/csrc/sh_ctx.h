@@ -82,6 +82,7 @@ struct sh_state {
 struct sh_ctx {
     int device = 0;
     hipStream_t stream = nullptr;
+    bool own_stream = true;          // false: the caller's (sh_create_on), null for the default stream
     hipEvent_t ev0 = nullptr, ev1 = nullptr;
     bool loaded = false;
     sh_model_info info{};

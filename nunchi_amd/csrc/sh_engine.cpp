@@ -456,7 +456,7 @@ extern "C" {
 
 const char* sh_last_error(void) { return g_err.c_str(); }
 
-int sh_create(int device, sh_ctx** out) {
+static int create(int device, bool own_stream, hipStream_t stream, sh_ctx** out) {
     if (!out) return fail(SH_E_ARG, "sh_create: out is null");
     int n = 0;
     HIPCHK(hipGetDeviceCount(&n));
@@ -466,14 +466,16 @@ int sh_create(int device, sh_ctx** out) {
     if (rs != SH_OK) return rs;
     auto c = std::make_unique<sh_ctx>();
     c->device = device;
-    HIPCHK(hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking));
+    c->own_stream = own_stream;
+    if (own_stream) HIPCHK(hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking));
+    else c->stream = stream;
     HIPCHK(hipEventCreate(&c->ev0));
     HIPCHK(hipEventCreate(&c->ev1));
     HIPCHK(hipHostMalloc((void**)&c->P_host, sizeof(step_params), hipHostMallocDefault));
     HIPCHK(hipMalloc((void**)&c->P_dev, sizeof(step_params)));
     memset(c->P_host, 0, sizeof(step_params));
     const char* g = getenv("SEOUL_HIP_GRAPHS");
-    c->use_graphs = !(g && g[0] == '0');
+    c->use_graphs = !(g && g[0] == '0') && (own_stream || stream);   // (the default stream cannot be captured)
     const char* pf = getenv("SEOUL_HIP_PREFILL");
     c->use_prefill = !(pf && strcmp(pf, "0") == 0);
     const char* pc = getenv("SEOUL_HIP_PRECUT");
@@ -482,10 +484,13 @@ int sh_create(int device, sh_ctx** out) {
     return SH_OK;
 }
 
+int sh_create(int device, sh_ctx** out) { return create(device, true, nullptr, out); }
+int sh_create_on(int device, void* stream, sh_ctx** out) { return create(device, false, static_cast<hipStream_t>(stream), out); }
+
 int sh_destroy(sh_ctx* c) {
     if (!c) return SH_OK;
     (void)hipSetDevice(c->device);
-    if (c->stream) (void)hipStreamSynchronize(c->stream);
+    if (c->stream || !c->own_stream) (void)hipStreamSynchronize(c->stream);
     for (sh_state* s : c->states) { release_state_memory(s); s->ctx = nullptr; }   // handles stay valid, detached
     for (sh_q4* t : c->tables) { if (t->mem) (void)hipFree(t->mem); t->mem = nullptr; t->ctx = nullptr; }
     for (auto& row : c->graph)
@@ -501,7 +506,7 @@ int sh_destroy(sh_ctx* c) {
     if (c->gen_out) (void)hipFree(c->gen_out);
     if (c->ev0) (void)hipEventDestroy(c->ev0);
     if (c->ev1) (void)hipEventDestroy(c->ev1);
-    if (c->stream) (void)hipStreamDestroy(c->stream);
+    if (c->stream && c->own_stream) (void)hipStreamDestroy(c->stream);
     delete c;
     return SH_OK;
 }

@@ -1,0 +1,503 @@
+// Attention of a batch of conversations over keys and values in pages: positions that all requests share, read once as
+// one matrix product for all query rows, and each request's own. Parts of the keys are taken by workgroups of their own
+// (k_page_attn) and joined after them (k_page_join): with a part's maximum m, sum l of e^(s - m) and sum O of e^(s - m) v,
+// two parts have m' = max(m1, m2), l' = l1 e^(m1 - m') + l2 e^(m2 - m'), O' likewise, and the result is O / l.
+#include <hip/hip_runtime.h>
+
+#include <climits>
+
+#include "sh_device.h"
+#include "sh_serve.h"
+
+namespace sh {
+namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+template <class T> struct mat;
+template <> struct mat<_Float16> {
+    static constexpr unsigned EXP = 0x7C00u;   // the exponent bits of one value: all set in infinities and NaN
+    static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct mat<__bf16> {
+    static constexpr unsigned EXP = 0x7F80u;
+    static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <class T> __device__ __forceinline__ unsigned pack2(float x, float y) {
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    const t2 v = {(T)x, (T)y};   // to nearest
+    return __builtin_bit_cast(unsigned, v);
+}
+template <class T> __device__ __forceinline__ float of_bits(unsigned h) {
+    return (float)__builtin_bit_cast(T, (unsigned short)h);
+}
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+// e^(from - to) in powers of two for maxima that may be -inf (nothing seen yet)
+__device__ __forceinline__ float rescale(float from, float to) { return from == -INFINITY ? 0.0f : exp2_(from - to); }
+
+template <class F> __device__ __forceinline__ int over16(int v, F f) {   // the same value in the 16 lanes of a column group
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v = f(v, __shfl_xor(v, o));
+    return v;
+}
+
+template <int D, int NT> constexpr int out_pitch() { return D + 4; }   // floats per column in LDS (banks shift by 4)
+
+// Columns: the (row, query head) pairs of one kv head, packed; a workgroup takes 16 NT of them and one part of the keys,
+// its four waves take blocks of 32 keys in turn. With K of 32 keys as rows of the first product (S^T = K Q^T) a lane
+// holds the scores of one column, so maxima and sums stay in the lane; rows are dealt to the product so that a lane's
+// eight scores are eight neighbouring keys, which are its operand of the second product (O^T = V^T P^T) as they are.
+// V's operand is eight keys of one dimension: each lane loads the same D / 16 dimensions of eight keys and turns the
+// block with byte permutes. Nothing passes through LDS before the waves are joined. Weights are rounded to the values'
+// 16 bits for the second product, relative to a maximum that is at most 2^8 behind the true one (the accumulators are
+// rescaled only when a score passes it by more): their sum stays in 32 bits.
+template <class T, int D, int NT, bool SHARED>
+__global__ __launch_bounds__(256) void k_page_attn(pattn_args a) {
+    constexpr int NC = 16 * NT, E = D / 16, CH = D / 32, VW = E / 2, PITCH = out_pitch<D, NT>();
+    __shared__ __align__(16) float o_s[2][NC * PITCH];
+    __shared__ float ml_s[2][2][NC];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m16 = lane & 15, quad = lane >> 4;
+    const int S = SHARED ? a.sp : a.so, per = a.n_kv * S;
+    const int gs = blockIdx.x % per, g = gs % a.n_kv, part = gs / a.n_kv;
+    const int tile = blockIdx.x / per;
+    // ---- the workgroup's columns ----
+    int i = 0, r0 = 0, r1, ct = tile;      // request, its rows, tile of columns within them
+    if constexpr (SHARED) {
+        r1 = a.cu ? min(max(a.cu[a.n], 0), a.rows) : a.rows;
+    } else if (!a.cu) {
+        const int tpr = (a.grp + NC - 1) / NC;
+        i = tile / tpr;
+        ct = tile - i * tpr;
+        r0 = i;
+        r1 = i + 1;
+    } else {
+        // request i owns the tiles first(i) .. first(i + 1) - 1, at least as many as its columns fill
+        auto row_at = [&](int k) { return min(max(a.cu[k], 0), a.rows); };
+        auto first = [&](int k) { return (int)((long long)row_at(k) * a.grp / NC) + k; };
+        int lo = 0, hi = a.n;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (first(mid) <= tile) lo = mid;
+            else hi = mid;
+        }
+        i = lo;
+        ct = tile - first(i);
+        r0 = row_at(i);
+        r1 = min(row_at(i + 1), r0 + a.max_rows);
+    }
+    const int ncol = (r1 - r0) * a.grp, c0 = ct * NC;
+    if (c0 < 0 || c0 >= ncol) return;
+    // ---- what each column sees: keys lo .. hi - 1 of this part of the cache ----
+    int row[NT], head[NT], lo[NT], hi[NT];
+    bool live[NT];
+    const int own_max = min((long long)a.max_len, (long long)a.cols << a.page_log);
+    int lo0 = INT_MAX, lo1 = 0, hi0 = INT_MAX, hi1 = 0;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const int c = c0 + 16 * t + m16, cc = min(c, ncol - 1);
+        live[t] = c < ncol;
+        row[t] = r0 + cc / a.grp;
+        head[t] = g * a.grp + cc % a.grp;
+        int at = 0;                        // the row's own position
+        if (!SHARED || a.window) {
+            int k = i, first_row = r0, rows_k = r1 - r0;
+            if (SHARED) {
+                if (a.cu) {                // the row's request
+                    int x = 0, y = a.n;
+                    while (y - x > 1) {
+                        const int mid = (x + y) >> 1;
+                        if (a.cu[mid] <= row[t]) x = mid;
+                        else y = mid;
+                    }
+                    k = x;
+                    first_row = a.cu[k];
+                    rows_k = a.cu[k + 1] - first_row;
+                } else {
+                    k = first_row = row[t];
+                    rows_k = 1;
+                }
+            } else if (a.cu) {
+                rows_k = a.cu[i + 1] - a.cu[i];
+            }
+            // (at most its last place: row starts that contradict each other lead nowhere else)
+            at = (int)min(min(max(a.len[k], 0), own_max) - (long long)rows_k + (row[t] - first_row), own_max - 1ll);
+        }
+        lo[t] = 0;
+        if constexpr (SHARED) {
+            hi[t] = a.prefix_len;
+            if (a.window) lo[t] = min(max(a.prefix_len + at + 1 - a.window, 0), a.prefix_len);
+        } else {
+            hi[t] = max(at + 1, 0);
+            if (a.window) lo[t] = max(at + 1 - a.window, 0);
+        }
+        lo0 = min(lo0, lo[t]);
+        lo1 = max(lo1, lo[t]);
+        hi0 = min(hi0, hi[t]);
+        hi1 = max(hi1, hi[t]);
+    }
+    auto mn = [](int x, int y) { return min(x, y); };
+    auto mx = [](int x, int y) { return max(x, y); };
+    lo0 = __builtin_amdgcn_readfirstlane(over16(lo0, mn));
+    lo1 = __builtin_amdgcn_readfirstlane(over16(lo1, mx));
+    hi0 = __builtin_amdgcn_readfirstlane(over16(hi0, mn));
+    hi1 = __builtin_amdgcn_readfirstlane(over16(hi1, mx));
+    // ---- the part: the first starts where the first column does; the last goes to the end ----
+    const int chunk = SHARED ? a.pchunk : a.ochunk;
+    const long long k0l = (long long)(lo0 & ~31) + (long long)part * chunk;
+    const int k1 = part + 1 == S ? hi1 : (int)min((long long)hi1, k0l + chunk);
+    const bool any = k0l < k1;
+    const int k0 = any ? (int)k0l : 0;
+
+    f32x4 o[E][NT];
+    float m[NT], l[NT];
+    u32x4 qf[CH][NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        m[t] = -INFINITY;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e][t] = f32x4{0, 0, 0, 0};
+    }
+    if (any) {
+        const T* qp = (const T*)a.q;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int c = 0; c < CH; c++)
+                qf[c][t] = *(const u32x4*)(qp + ((size_t)row[t] * a.n_head + head[t]) * D + c * 32 + quad * 8);
+        const int32_t* tab = SHARED ? a.prefix : a.table + (size_t)i * a.cols;
+        const int pl = a.page_log, pm = (1 << pl) - 1, last = hi1 - 1;
+        const size_t page_sz = ((size_t)a.n_kv << pl) * D;
+        const T* kp = (const T*)a.keys + ((size_t)g << pl) * D;
+        const T* vp = (const T*)a.values + ((size_t)g << pl) * D;
+        const int koff = ((m16 >> 2) << 3) + (m16 & 3);
+        for (int kt = k0 + 32 * wv; kt < k1; kt += 128) {
+            // a block of 32 keys lies in one page, or in two of 16
+            const int id0 = tab[kt >> pl], id1 = pl == 4 ? tab[min(kt + 16, last) >> 4] : id0;
+            const bool ok0 = (unsigned)id0 < (unsigned)a.n_pages, ok1 = (unsigned)id1 < (unsigned)a.n_pages;
+            const size_t b0 = (ok0 ? (size_t)id0 : 0) * page_sz, b1 = (ok1 ? (size_t)id1 : 0) * page_sz;
+            auto at = [&](int off) {       // place of key kt + off (the last one where it is past the end)
+                const int f = min(off, last - kt);
+                return pl == 4 ? ((f & 16) ? b1 : b0) + (size_t)(f & 15) * D : b0 + (size_t)((kt & pm) + f) * D;
+            };
+            u32x4 kf[2][CH];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const T* p = kp + at(koff + 4 * t) + quad * 8;
+#pragma unroll
+                for (int c = 0; c < CH; c++) kf[t][c] = *(const u32x4*)(p + c * 32);
+            }
+            unsigned vw[8][VW];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const T* p = vp + at(quad * 8 + k) + m16 * E;
+                if constexpr (VW == 4) *(u32x4*)vw[k] = *(const u32x4*)p;
+                else if constexpr (VW == 2) *(uint2*)vw[k] = *(const uint2*)p;
+                else vw[k][0] = *(const unsigned*)p;
+            }
+            const bool full = kt >= lo1 && kt + 32 <= hi0 && ok0 && ok1;
+            const bool mine = quad >= 2 ? ok1 : ok0;
+            unsigned pw[NT][4];
+            float ps[NT][8];
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                float x[8];
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    f32x4 s = {0, 0, 0, 0};
+#pragma unroll
+                    for (int c = 0; c < CH; c++) s = mat<T>::mul(kf[b][c], qf[c][t], s);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) x[4 * b + r] = s[r] * a.c;
+                }
+                if (!full) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const int key = kt + quad * 8 + k;
+                        x[k] = mine && key >= lo[t] && key < hi[t] ? x[k] : -INFINITY;
+                    }
+                }
+                float top = x[0];
+#pragma unroll
+                for (int k = 1; k < 8; k++) top = fmaxf(top, x[k]);
+                if (__any(top > m[t] + 8.0f)) {
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const float to = fmaxf(m[t], top), f = rescale(m[t], to);
+                    l[t] *= f;
+#pragma unroll
+                    for (int e = 0; e < E; e++) o[e][t] *= f;
+                    m[t] = to;
+                }
+                const float ref = m[t] == -INFINITY ? 0.0f : m[t];
+                float sum = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    ps[t][k] = exp2_(x[k] - ref);
+                    sum += ps[t][k];
+                }
+                l[t] += sum;
+#pragma unroll
+                for (int k = 0; k < 4; k++) pw[t][k] = pack2<T>(ps[t][2 * k], ps[t][2 * k + 1]);
+            }
+            bool odd = false;              // infinities or NaN among the values of a block that columns see in part
+            if (!full) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const int key = kt + quad * 8 + k;
+                    const bool seen = mine && key >= lo0 && key < hi1;
+#pragma unroll
+                    for (int w = 0; w < VW; w++) {
+                        vw[k][w] = seen ? vw[k][w] : 0u;
+                        odd |= (vw[k][w] & mat<T>::EXP) == mat<T>::EXP || ((vw[k][w] >> 16) & mat<T>::EXP) == mat<T>::EXP;
+                    }
+                }
+                if (__any(odd)) {
+                    // A weight of 0 times an infinity would reach columns that do not see the key: such values are
+                    // left out of the product and added to the columns that do, key by key
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+#pragma unroll
+                        for (int w = 0; w < VW; w++) {
+                            if ((vw[k][w] & mat<T>::EXP) == mat<T>::EXP) vw[k][w] &= 0xFFFF0000u;
+                            if (((vw[k][w] >> 16) & mat<T>::EXP) == mat<T>::EXP) vw[k][w] &= 0x0000FFFFu;
+                        }
+                        for (int kq = 0; kq < 4; kq++) {
+                            const int key = kt + kq * 8 + k;
+                            const bool there = (kq >= 2 ? ok1 : ok0) && key < hi1;
+                            const T* p = vp + at(kq * 8 + k) + quad * 4 * E;   // this lane's dimensions of O
+#pragma unroll
+                            for (int t = 0; t < NT; t++) {
+                                const float w = __shfl(ps[t][k], kq * 16 + m16);
+                                if (!there || key < lo[t] || key >= hi[t]) continue;
+#pragma unroll
+                                for (int r = 0; r < 4; r++)
+#pragma unroll
+                                    for (int e = 0; e < E; e++) {
+                                        const float v = (float)p[r * E + e];
+                                        if (!(fabsf(v) < INFINITY)) o[e][t][r] += w * v;
+                                    }
+                            }
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < E; e++) {  // dimension m16 * E + e of eight keys
+                const unsigned sel = (e & 1) ? 0x07060302u : 0x05040100u;
+                u32x4 vf;
+#pragma unroll
+                for (int k = 0; k < 4; k++) vf[k] = __builtin_amdgcn_perm(vw[2 * k + 1][e >> 1], vw[2 * k][e >> 1], sel);
+#pragma unroll
+                for (int t = 0; t < NT; t++) o[e][t] = mat<T>::mul(vf, u32x4{pw[t][0], pw[t][1], pw[t][2], pw[t][3]}, o[e][t]);
+            }
+        }
+    }
+    // ---- the four waves joined: 2 and 3 into 0 and 1, then 1 into 0 ----
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        l[t] += __shfl_xor(l[t], 16);
+        l[t] += __shfl_xor(l[t], 32);
+    }
+#pragma unroll
+    for (int step = 2; step > 0; step >>= 1) {
+        if (wv >= step && wv < 2 * step) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const int c = 16 * t + m16;
+                if (quad == 0) {
+                    ml_s[wv - step][0][c] = m[t];
+                    ml_s[wv - step][1][c] = l[t];
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int e = 0; e < E; e++) o_s[wv - step][c * PITCH + (quad * 4 + r) * E + e] = o[e][t][r];
+            }
+        }
+        __syncthreads();
+        if (wv < step) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const int c = 16 * t + m16;
+                const float m2 = ml_s[wv][0][c], l2 = ml_s[wv][1][c];
+                const float to = fmaxf(m[t], m2), f1 = rescale(m[t], to), f2 = rescale(m2, to);
+                m[t] = to;
+                l[t] = l[t] * f1 + l2 * f2;
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+                        o[e][t][r] = o[e][t][r] * f1 + o_s[wv][c * PITCH + (quad * 4 + r) * E + e] * f2;
+            }
+        }
+        __syncthreads();
+    }
+    if (wv) return;
+    const bool alone = a.sp + a.so == 1;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        if (!live[t]) continue;
+        const size_t rh = (size_t)row[t] * a.n_head + head[t];
+        if (alone) {
+            float f = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+            if (a.gate) f *= 1.0f / (1.0f + expf(-a.gate[rh]));
+            unsigned* dst = (unsigned*)((T*)a.out + rh * D + quad * 4 * E);
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int e = 0; e < E; e += 2) {
+                    const float x = o[e][t][r], y = o[e + 1][t][r];
+                    dst[(r * E + e) / 2] = l[t] == 0.0f ? 0u : pack2<T>(x * f, y * f);
+                }
+            if (a.lse && quad == 0) a.lse[rh] = l[t] == 0.0f ? -INFINITY : (m[t] + log2f(l[t])) * 0.69314718055994531f;
+        } else {
+            const size_t at = (size_t)(SHARED ? part : a.sp + part) * a.rows * a.n_head + rh;
+            if (quad == 0) a.part_ml[at] = make_float2(m[t], l[t]);
+            if (any) {
+                float* dst = a.part_o + at * D + quad * 4 * E;
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int e = 0; e < E; e++) dst[r * E + e] = o[e][t][r];
+            }
+        }
+    }
+}
+
+// One workgroup per (row, query head): waves take parts in turn, each lane the dimensions lane + 64 k
+template <class T, int D>
+__global__ __launch_bounds__(256) void k_page_join(pattn_args a) {
+    constexpr int PL = D > 64 ? D / 64 : 1;
+    __shared__ float o_s[4][D];
+    __shared__ float l_s[4];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, parts = a.sp + a.so;
+    const size_t rh = blockIdx.x, stride = (size_t)a.rows * a.n_head;
+    const int row = (int)(rh / a.n_head);
+    if (a.cu) {   // rows behind the last request, and those past max_rows of theirs, have no parts
+        int x = 0, y = a.n;
+        while (y - x > 1) {
+            const int mid = (x + y) >> 1;
+            if (a.cu[mid] <= row) x = mid;
+            else y = mid;
+        }
+        const int first = max(a.cu[x], 0);
+        if (row < first || row >= a.cu[x + 1] || row - first >= a.max_rows) return;
+    }
+    float m = -INFINITY;
+    for (int p = lane; p < parts; p += 64) {
+        const float2 ml = a.part_ml[p * stride + rh];
+        if (ml.y != 0.0f) m = fmaxf(m, ml.x);
+    }
+    m = wave_max(m);
+    float l = 0.0f, o[PL] = {};
+    for (int p = wv; p < parts; p += 4) {
+        const float2 ml = a.part_ml[p * stride + rh];
+        if (ml.y == 0.0f) continue;
+        const float f = exp2_(ml.x - m);
+        l += ml.y * f;
+#pragma unroll
+        for (int k = 0; k < PL; k++)
+            if (lane + 64 * k < D) o[k] = fmaf(a.part_o[(p * stride + rh) * D + lane + 64 * k], f, o[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < PL; k++)
+        if (lane + 64 * k < D) o_s[wv][lane + 64 * k] = o[k];
+    if (lane == 0) l_s[wv] = l;
+    __syncthreads();
+    l = (l_s[0] + l_s[1]) + (l_s[2] + l_s[3]);
+    float f = l == 0.0f ? 0.0f : 1.0f / l;
+    if (a.gate) f *= 1.0f / (1.0f + expf(-a.gate[rh]));
+    if (threadIdx.x < D) {
+        const int d = threadIdx.x;
+        const float x = (o_s[0][d] + o_s[1][d]) + (o_s[2][d] + o_s[3][d]);
+        ((T*)a.out)[rh * D + d] = (T)(l == 0.0f ? 0.0f : x * f);
+    }
+    if (a.lse && threadIdx.x == 0) a.lse[rh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+}
+
+// column groups of 16 per workgroup: as many as the columns fill, up to what the registers hold
+int col_groups(int D, long long cols) {
+    const int most = D > 64 ? 2 : 4;
+    return cols <= 16 ? 1 : cols <= 32 || most == 2 ? 2 : 4;
+}
+
+long long shared_tiles(const pattn_args& a, int nt) { return ((long long)a.rows * a.grp + 16 * nt - 1) / (16 * nt); }
+long long own_tiles(const pattn_args& a, int nt, bool single) {
+    return single ? (long long)a.n * ((a.grp + 16 * nt - 1) / (16 * nt)) : (long long)a.rows * a.grp / (16 * nt) + a.n;
+}
+
+template <class T, int D, int NT> hipError_t run_shared(const pattn_args& a, hipStream_t s) {
+    k_page_attn<T, D, NT, true><<<dim3((unsigned)(shared_tiles(a, NT) * a.n_kv * a.sp)), 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+template <class T, int D, int NT> hipError_t run_own(const pattn_args& a, hipStream_t s) {
+    k_page_attn<T, D, NT, false><<<dim3((unsigned)(own_tiles(a, NT, !a.cu) * a.n_kv * a.so)), 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+template <class T, int D> hipError_t run_all(const pattn_args& a, hipStream_t s) {
+    hipError_t e = hipSuccess;
+    if (a.sp) {
+        const int nt = col_groups(D, (long long)a.rows * a.grp);
+        if (nt == 1) e = run_shared<T, D, 1>(a, s);
+        else if (nt == 2) e = run_shared<T, D, 2>(a, s);
+        else if constexpr (D <= 64) e = run_shared<T, D, 4>(a, s);
+        if (e != hipSuccess) return e;
+    }
+    const int nt = col_groups(D, (long long)a.max_rows * a.grp);
+    if (nt == 1) e = run_own<T, D, 1>(a, s);
+    else if (nt == 2) e = run_own<T, D, 2>(a, s);
+    else if constexpr (D <= 64) e = run_own<T, D, 4>(a, s);
+    if (e != hipSuccess || a.sp + a.so == 1) return e;
+    k_page_join<T, D><<<dim3((unsigned)((long long)a.rows * a.n_head)), 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+template <class T> hipError_t run_dim(int D, const pattn_args& a, hipStream_t s) {
+    return D == 32 ? run_all<T, 32>(a, s) : D == 64 ? run_all<T, 64>(a, s) : run_all<T, 128>(a, s);
+}
+
+void split(long long base, long long range, int* parts, int* chunk) {
+    long long p = 1024 / (base > 0 ? base : 1), most = (range + 255) / 256;
+    if (p > most) p = most;
+    if (p < 1) p = 1;
+    const long long c = ((range + p - 1) / p + 127) / 128 * 128;
+    *chunk = (int)(c < 128 ? 128 : c);
+    *parts = (int)((range + *chunk - 1) / *chunk);
+    if (*parts < 1) *parts = 1;
+}
+
+}  // namespace
+
+// Parts so that about four workgroups per compute unit run, of 256 keys or more.
+bool page_attn_split(int D, bool single, pattn_args& a) {
+    a.sp = a.pchunk = 0;
+    long long blocks = (long long)a.rows * a.n_head;
+    if (a.prefix_len) {
+        const long long range = a.window && a.window + 31ll < a.prefix_len ? a.window + 31ll : a.prefix_len;
+        const long long base = shared_tiles(a, col_groups(D, (long long)a.rows * a.grp)) * a.n_kv;
+        split(base, range, &a.sp, &a.pchunk);
+        if (base * a.sp > blocks) blocks = base * a.sp;
+    }
+    const int nt = col_groups(D, (long long)a.max_rows * a.grp);
+    long long range = a.max_len;
+    if (a.window) {
+        const long long rows = 16ll * nt / a.grp + 2, seen = a.window + 31ll + (rows < a.max_rows ? rows : a.max_rows);
+        if (seen < range) range = seen;
+    }
+    const long long base = own_tiles(a, nt, single) * a.n_kv;
+    split(base, range, &a.so, &a.ochunk);
+    if (base * a.so > blocks) blocks = base * a.so;
+    // (columns of one kv head are counted in 32 bits in the kernel)
+    return blocks <= INT_MAX && (long long)a.rows * a.grp <= INT_MAX / 2;
+}
+
+hipError_t launch_page_attn(int D, int type, const pattn_args& a, hipStream_t s) {
+    return type == TY_F16 ? run_dim<_Float16>(D, a, s) : run_dim<__bf16>(D, a, s);
+}
+
+}  // namespace sh
