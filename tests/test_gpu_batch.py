@@ -623,6 +623,24 @@ def test_sample(ctx, vocab, kind, kw):
     check_sample(ctx, x, u, **kw)
 
 
+@pytest.mark.parametrize("vocab", [1000, 16384, 16385, 40000, 98304, 98305])
+def test_sample_more_than_are_allowed(ctx, vocab):
+    """top_k between the words that are allowed and all words, alone and with the other filters."""
+    x, u = random_scores(vocab, 5, vocab, banned=0.5)
+    for kw in (dict(top_k=int(0.7 * vocab)), dict(top_k=int(0.7 * vocab), top_p=0.8), dict(top_k=int(0.4 * vocab), top_p=0.95, min_p=0.001), dict(top_p=0.9)):
+        check_sample(ctx, x, u, **kw)
+
+
+@pytest.mark.parametrize("spread,temp", [(0.01, 1.0), (0.5, 3.0), (30.0, 1.0), (1000.0, 0.5), (1e30, 1e30), (1e-20, 1e-21)])
+def test_sample_scales(ctx, spread, temp):
+    """Weights that are nearly equal (cuts keep most words), and scores far apart."""
+    g = torch.Generator().manual_seed(3)
+    x = (spread * torch.randn(6, 30011, generator=g)).cuda()
+    u = torch.rand(6, generator=g, dtype=torch.float64).numpy()
+    for kw in (dict(), dict(top_k=900), dict(top_k=6000), dict(top_p=0.97), dict(top_k=20, top_p=0.7), dict(min_p=0.2)):
+        check_sample(ctx, x, u, temp=temp, **kw)
+
+
 def test_sample_largest_vocab(ctx):
     x, u = random_scores(1, 3, 524288)
     for kw in (dict(), dict(top_p=0.95), dict(top_k=100000), dict(top_k=70, top_p=0.9)):
