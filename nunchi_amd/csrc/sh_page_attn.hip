@@ -45,10 +45,27 @@ template <class F> __device__ __forceinline__ int over16(int v, F f) {   // the 
     for (int o = 8; o > 0; o >>= 1) v = f(v, __shfl_xor(v, o));
     return v;
 }
+// the request whose rows hold `row` (the last k with cu[k] <= row)
+__device__ __forceinline__ int request_of(const int32_t* cu, int n, int row) {
+    int x = 0, y = n;
+    while (y - x > 1) {
+        const int mid = (x + y) >> 1;
+        if (cu[mid] <= row) x = mid;
+        else y = mid;
+    }
+    return x;
+}
 
-template <int D, int NT> constexpr int out_pitch() { return D + 4; }   // floats per column in LDS (banks shift by 4)
+// what the four waves of a workgroup pass each other when they are joined: 16 NT columns of D sums (the pitch shifts
+// columns by four banks), maxima and sums of weights, of two waves
+template <int D, int NT> struct join_space {
+    static constexpr int NC = 16 * NT, PITCH = D + 4;
+    float o[2][NC * PITCH];
+    float m[2][NC], l[2][NC];
+};
 
-// Columns: the (row, query head) pairs of one kv head, packed; a workgroup takes 16 NT of them and one part of the keys,
+// Keys are counted along one line: the shared positions, a gap to the next multiple of 32, the request's own.
+// Columns: the (row, query head) pairs of one kv head, packed; a workgroup takes 16 NT of them and one part of the line,
 // its four waves take blocks of 32 keys in turn. With K of 32 keys as rows of the first product (S^T = K Q^T) a lane
 // holds the scores of one column, so maxima and sums stay in the lane; rows are dealt to the product so that a lane's
 // eight scores are eight neighbouring keys, which are its operand of the second product (O^T = V^T P^T) as they are.
@@ -56,15 +73,16 @@ template <int D, int NT> constexpr int out_pitch() { return D + 4; }   // floats
 // block with byte permutes. Nothing passes through LDS before the waves are joined. Weights are rounded to the values'
 // 16 bits for the second product, relative to a maximum that is at most 2^8 behind the true one (the accumulators are
 // rescaled only when a score passes it by more): their sum stays in 32 bits.
+// SHARED: the columns of all requests over the shared positions. Else one request's columns over its own positions, and
+// over the shared ones before them where no SHARED part takes them (a.fused).
 template <class T, int D, int NT, bool SHARED>
-__global__ __launch_bounds__(256) void k_page_attn(pattn_args a) {
-    constexpr int NC = 16 * NT, E = D / 16, CH = D / 32, VW = E / 2, PITCH = out_pitch<D, NT>();
-    __shared__ __align__(16) float o_s[2][NC * PITCH];
-    __shared__ float ml_s[2][2][NC];
+__device__ __forceinline__ void attend(const pattn_args& a, const int block, join_space<D, NT>& js) {
+    constexpr int NC = 16 * NT, E = D / 16, CH = D / 32, VW = E / 2, PITCH = join_space<D, NT>::PITCH;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m16 = lane & 15, quad = lane >> 4;
     const int S = SHARED ? a.sp : a.so, per = a.n_kv * S;
-    const int gs = blockIdx.x % per, g = gs % a.n_kv, part = gs / a.n_kv;
-    const int tile = blockIdx.x / per;
+    // (workgroups of the same keys are `per` apart: on one XCD where that is a multiple of 8)
+    const int gs = block % per, g = gs % a.n_kv, part = gs / a.n_kv;
+    const int tile = block / per;
     // ---- the workgroup's columns ----
     int i = 0, r0 = 0, r1, ct = tile;      // request, its rows, tile of columns within them
     if constexpr (SHARED) {
@@ -92,10 +110,11 @@ __global__ __launch_bounds__(256) void k_page_attn(pattn_args a) {
     }
     const int ncol = (r1 - r0) * a.grp, c0 = ct * NC;
     if (c0 < 0 || c0 >= ncol) return;
-    // ---- what each column sees: keys lo .. hi - 1 of this part of the cache ----
+    // ---- what each column sees: keys lo .. hi - 1 of the line, the gap left out ----
+    const int L0 = a.prefix_len, P = a.own_at;
     int row[NT], head[NT], lo[NT], hi[NT];
     bool live[NT];
-    const int own_max = min((long long)a.max_len, (long long)a.cols << a.page_log);
+    const int own_max = (int)min((long long)a.max_len, (long long)a.cols << a.page_log);
     int lo0 = INT_MAX, lo1 = 0, hi0 = INT_MAX, hi1 = 0;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
@@ -103,37 +122,21 @@ __global__ __launch_bounds__(256) void k_page_attn(pattn_args a) {
         live[t] = c < ncol;
         row[t] = r0 + cc / a.grp;
         head[t] = g * a.grp + cc % a.grp;
-        int at = 0;                        // the row's own position
+        int at = 0;                        // the row's own position, counted from the first that is not shared
         if (!SHARED || a.window) {
-            int k = i, first_row = r0, rows_k = r1 - r0;
-            if (SHARED) {
-                if (a.cu) {                // the row's request
-                    int x = 0, y = a.n;
-                    while (y - x > 1) {
-                        const int mid = (x + y) >> 1;
-                        if (a.cu[mid] <= row[t]) x = mid;
-                        else y = mid;
-                    }
-                    k = x;
-                    first_row = a.cu[k];
-                    rows_k = a.cu[k + 1] - first_row;
-                } else {
-                    k = first_row = row[t];
-                    rows_k = 1;
-                }
-            } else if (a.cu) {
-                rows_k = a.cu[i + 1] - a.cu[i];
-            }
+            const int k = !SHARED ? i : a.cu ? request_of(a.cu, a.n, row[t]) : row[t];
+            const int first_row = a.cu ? a.cu[k] : k, rows_k = a.cu ? a.cu[k + 1] - first_row : 1;
             // (at most its last place: row starts that contradict each other lead nowhere else)
             at = (int)min(min(max(a.len[k], 0), own_max) - (long long)rows_k + (row[t] - first_row), own_max - 1ll);
         }
-        lo[t] = 0;
+        // the first position of the line that a window leaves
+        const int from = a.window ? L0 + at + 1 - a.window : 0;
         if constexpr (SHARED) {
-            hi[t] = a.prefix_len;
-            if (a.window) lo[t] = min(max(a.prefix_len + at + 1 - a.window, 0), a.prefix_len);
+            lo[t] = min(max(from, 0), L0);
+            hi[t] = L0;
         } else {
-            hi[t] = max(at + 1, 0);
-            if (a.window) lo[t] = max(at + 1 - a.window, 0);
+            lo[t] = from >= L0 ? P + (from - L0) : a.fused ? max(from, 0) : P;
+            hi[t] = at >= 0 ? P + at + 1 : a.fused ? L0 : P;
         }
         lo0 = min(lo0, lo[t]);
         lo1 = max(lo1, lo[t]);
@@ -170,20 +173,24 @@ __global__ __launch_bounds__(256) void k_page_attn(pattn_args a) {
 #pragma unroll
             for (int c = 0; c < CH; c++)
                 qf[c][t] = *(const u32x4*)(qp + ((size_t)row[t] * a.n_head + head[t]) * D + c * 32 + quad * 8);
-        const int32_t* tab = SHARED ? a.prefix : a.table + (size_t)i * a.cols;
-        const int pl = a.page_log, pm = (1 << pl) - 1, last = hi1 - 1;
+        const int32_t* own = SHARED ? nullptr : a.table + (size_t)i * a.cols;
+        const int pl = a.page_log, pm = (1 << pl) - 1;
         const size_t page_sz = ((size_t)a.n_kv << pl) * D;
         const T* kp = (const T*)a.keys + ((size_t)g << pl) * D;
         const T* vp = (const T*)a.values + ((size_t)g << pl) * D;
         const int koff = ((m16 >> 2) << 3) + (m16 & 3);
         for (int kt = k0 + 32 * wv; kt < k1; kt += 128) {
-            // a block of 32 keys lies in one page, or in two of 16
-            const int id0 = tab[kt >> pl], id1 = pl == 4 ? tab[min(kt + 16, last) >> 4] : id0;
+            // a block of 32 keys lies in one page, or in two of 16; behind `last` of its table there are none
+            const bool in_shared = SHARED || kt < P;
+            const int32_t* tab = in_shared ? a.prefix : own;
+            const int k_at = in_shared ? kt : kt - P, last = in_shared ? L0 - 1 : hi1 - 1 - P, ahead = last - k_at;
+            if (!SHARED && ahead < 0) continue;   // (the gap alone)
+            const int id0 = tab[k_at >> pl], id1 = pl == 4 ? tab[min(k_at + 16, last) >> 4] : id0;
             const bool ok0 = (unsigned)id0 < (unsigned)a.n_pages, ok1 = (unsigned)id1 < (unsigned)a.n_pages;
             const size_t b0 = (ok0 ? (size_t)id0 : 0) * page_sz, b1 = (ok1 ? (size_t)id1 : 0) * page_sz;
             auto at = [&](int off) {       // place of key kt + off (the last one where it is past the end)
-                const int f = min(off, last - kt);
-                return pl == 4 ? ((f & 16) ? b1 : b0) + (size_t)(f & 15) * D : b0 + (size_t)((kt & pm) + f) * D;
+                const int f = min(off, ahead);
+                return pl == 4 ? ((f & 16) ? b1 : b0) + (size_t)(f & 15) * D : b0 + (size_t)((k_at & pm) + f) * D;
             };
             u32x4 kf[2][CH];
 #pragma unroll
@@ -200,10 +207,10 @@ __global__ __launch_bounds__(256) void k_page_attn(pattn_args a) {
                 else if constexpr (VW == 2) *(uint2*)vw[k] = *(const uint2*)p;
                 else vw[k][0] = *(const unsigned*)p;
             }
-            const bool full = kt >= lo1 && kt + 32 <= hi0 && ok0 && ok1;
+            const bool full = kt >= lo1 && kt + 32 <= hi0 && ahead >= 31 && ok0 && ok1;
             const bool mine = quad >= 2 ? ok1 : ok0;
+            const int end = kt + ahead + 1;
             unsigned pw[NT][4];
-            float ps[NT][8];
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 float x[8];
@@ -216,13 +223,14 @@ __global__ __launch_bounds__(256) void k_page_attn(pattn_args a) {
                     for (int r = 0; r < 4; r++) x[4 * b + r] = s[r] * a.c;
                 }
                 if (!full) {
+                    const int stop = min(hi[t], end);
 #pragma unroll
                     for (int k = 0; k < 8; k++) {
                         const int key = kt + quad * 8 + k;
-                        x[k] = mine && key >= lo[t] && key < hi[t] ? x[k] : -INFINITY;
+                        x[k] = mine && key >= lo[t] && key < stop ? x[k] : -INFINITY;
                     }
                 }
-                float top = x[0];
+                float top = x[0];          // (NaN is passed over)
 #pragma unroll
                 for (int k = 1; k < 8; k++) top = fmaxf(top, x[k]);
                 if (__any(top > m[t] + 8.0f)) {
@@ -238,19 +246,20 @@ __global__ __launch_bounds__(256) void k_page_attn(pattn_args a) {
                 float sum = 0.0f;
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
-                    ps[t][k] = exp2_(x[k] - ref);
-                    sum += ps[t][k];
+                    x[k] = exp2_(x[k] - ref);
+                    sum += x[k];
                 }
                 l[t] += sum;
 #pragma unroll
-                for (int k = 0; k < 4; k++) pw[t][k] = pack2<T>(ps[t][2 * k], ps[t][2 * k + 1]);
+                for (int k = 0; k < 4; k++) pw[t][k] = pack2<T>(x[2 * k], x[2 * k + 1]);
             }
-            bool odd = false;              // infinities or NaN among the values of a block that columns see in part
             if (!full) {
+                bool odd = false;          // infinities or NaN among the values of a block that columns see in part
+                const int stop = min(hi1, end);
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
                     const int key = kt + quad * 8 + k;
-                    const bool seen = mine && key >= lo0 && key < hi1;
+                    const bool seen = mine && key >= lo0 && key < stop;
 #pragma unroll
                     for (int w = 0; w < VW; w++) {
                         vw[k][w] = seen ? vw[k][w] : 0u;
@@ -269,11 +278,12 @@ __global__ __launch_bounds__(256) void k_page_attn(pattn_args a) {
                         }
                         for (int kq = 0; kq < 4; kq++) {
                             const int key = kt + kq * 8 + k;
-                            const bool there = (kq >= 2 ? ok1 : ok0) && key < hi1;
+                            const bool there = (kq >= 2 ? ok1 : ok0) && key < stop;
                             const T* p = vp + at(kq * 8 + k) + quad * 4 * E;   // this lane's dimensions of O
 #pragma unroll
                             for (int t = 0; t < NT; t++) {
-                                const float w = __shfl(ps[t][k], kq * 16 + m16);
+                                const unsigned two = __shfl(pw[t][k >> 1], kq * 16 + m16);
+                                const float w = of_bits<T>(k & 1 ? two >> 16 : two & 0xFFFFu);
                                 if (!there || key < lo[t] || key >= hi[t]) continue;
 #pragma unroll
                                 for (int r = 0; r < 4; r++)
@@ -306,18 +316,19 @@ __global__ __launch_bounds__(256) void k_page_attn(pattn_args a) {
     }
 #pragma unroll
     for (int step = 2; step > 0; step >>= 1) {
+        if (k0 + 32 * step >= k1) continue;   // (waves from `step` on had no block)
         if (wv >= step && wv < 2 * step) {
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 const int c = 16 * t + m16;
                 if (quad == 0) {
-                    ml_s[wv - step][0][c] = m[t];
-                    ml_s[wv - step][1][c] = l[t];
+                    js.m[wv - step][c] = m[t];
+                    js.l[wv - step][c] = l[t];
                 }
 #pragma unroll
                 for (int r = 0; r < 4; r++)
 #pragma unroll
-                    for (int e = 0; e < E; e++) o_s[wv - step][c * PITCH + (quad * 4 + r) * E + e] = o[e][t][r];
+                    for (int e = 0; e < E; e++) js.o[wv - step][c * PITCH + (quad * 4 + r) * E + e] = o[e][t][r];
             }
         }
         __syncthreads();
@@ -325,7 +336,7 @@ __global__ __launch_bounds__(256) void k_page_attn(pattn_args a) {
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 const int c = 16 * t + m16;
-                const float m2 = ml_s[wv][0][c], l2 = ml_s[wv][1][c];
+                const float m2 = js.m[wv][c], l2 = js.l[wv][c];
                 const float to = fmaxf(m[t], m2), f1 = rescale(m[t], to), f2 = rescale(m2, to);
                 m[t] = to;
                 l[t] = l[t] * f1 + l2 * f2;
@@ -333,7 +344,7 @@ __global__ __launch_bounds__(256) void k_page_attn(pattn_args a) {
                 for (int r = 0; r < 4; r++)
 #pragma unroll
                     for (int e = 0; e < E; e++)
-                        o[e][t][r] = o[e][t][r] * f1 + o_s[wv][c * PITCH + (quad * 4 + r) * E + e] * f2;
+                        o[e][t][r] = o[e][t][r] * f1 + js.o[wv][c * PITCH + (quad * 4 + r) * E + e] * f2;
             }
         }
         __syncthreads();
@@ -370,24 +381,43 @@ __global__ __launch_bounds__(256) void k_page_attn(pattn_args a) {
     }
 }
 
-// One workgroup per (row, query head): waves take parts in turn, each lane the dimensions lane + 64 k
-template <class T, int D>
+// waves per SIMD that the registers are to allow
+constexpr int waves_of(int D, int nts, int nto) { return nts > 1 || nto > 1 ? 2 : D > 64 ? 3 : 4; }
+
+// Shared and own parts in one launch, eight workgroups of either in turn (one for each XCD): the shared ones wait for the
+// matrix units, the own ones for memory, and together they take little longer than the longer of the two alone.
+template <class T, int D, int NTS, int NTO>
+__global__ __launch_bounds__(256, waves_of(D, NTS, NTO)) void k_page_attn(pattn_args a) {
+    __shared__ __align__(16) union { join_space<D, NTO> own; join_space<D, NTS ? NTS : 1> shared; } js;
+    int b = blockIdx.x;
+    if constexpr (NTS > 0) {
+        const long long grp = b >> 3, gs = (a.shared_blocks + 7) >> 3, all = gridDim.x >> 3;
+        const long long before = grp * gs / all, next = (grp + 1) * gs / all;   // shared groups before this one, with it
+        if (next > before) {
+            b = (int)(before * 8) + (b & 7);
+            if (b < a.shared_blocks) attend<T, D, NTS ? NTS : 1, true>(a, b, js.shared);
+            return;
+        }
+        b = (int)((grp - before) * 8) + (b & 7);
+        if (b >= a.own_blocks) return;
+    }
+    attend<T, D, NTO, false>(a, b, js.own);
+}
+
+// One wave per (row, query head), or all four for many parts: lanes take four dimensions each, as many parts at once as
+// fit a wave
+template <class T, int D, bool MANY>
 __global__ __launch_bounds__(256) void k_page_join(pattn_args a) {
-    constexpr int PL = D > 64 ? D / 64 : 1;
-    __shared__ float o_s[4][D];
+    constexpr int LP = D / 4, AT_ONCE = 64 / LP, WAVES = MANY ? 4 : 1;   // lanes per part, parts at once
+    __shared__ f32x4 o_s[MANY ? 4 : 1][LP];
     __shared__ float l_s[4];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, parts = a.sp + a.so;
-    const size_t rh = blockIdx.x, stride = (size_t)a.rows * a.n_head;
+    const size_t rh = MANY ? (size_t)blockIdx.x : (size_t)blockIdx.x * 4 + wv, stride = (size_t)a.rows * a.n_head;
+    if (rh >= stride) return;
     const int row = (int)(rh / a.n_head);
     if (a.cu) {   // rows behind the last request, and those past max_rows of theirs, have no parts
-        int x = 0, y = a.n;
-        while (y - x > 1) {
-            const int mid = (x + y) >> 1;
-            if (a.cu[mid] <= row) x = mid;
-            else y = mid;
-        }
-        const int first = max(a.cu[x], 0);
-        if (row < first || row >= a.cu[x + 1] || row - first >= a.max_rows) return;
+        const int k = request_of(a.cu, a.n, row), first = max(a.cu[k], 0);
+        if (row < first || row >= a.cu[k + 1] || row - first >= a.max_rows) return;
     }
     float m = -INFINITY;
     for (int p = lane; p < parts; p += 64) {
@@ -395,74 +425,74 @@ __global__ __launch_bounds__(256) void k_page_join(pattn_args a) {
         if (ml.y != 0.0f) m = fmaxf(m, ml.x);
     }
     m = wave_max(m);
-    float l = 0.0f, o[PL] = {};
-    for (int p = wv; p < parts; p += 4) {
+    float l = 0.0f;
+    f32x4 o = {0, 0, 0, 0};
+    const int d = (lane % LP) * 4;
+#pragma unroll 4
+    for (int p = (MANY ? wv * AT_ONCE : 0) + lane / LP; p < parts; p += WAVES * AT_ONCE) {
         const float2 ml = a.part_ml[p * stride + rh];
         if (ml.y == 0.0f) continue;
         const float f = exp2_(ml.x - m);
         l += ml.y * f;
-#pragma unroll
-        for (int k = 0; k < PL; k++)
-            if (lane + 64 * k < D) o[k] = fmaf(a.part_o[(p * stride + rh) * D + lane + 64 * k], f, o[k]);
+        o += *(const f32x4*)(a.part_o + (p * stride + rh) * D + d) * f;
     }
 #pragma unroll
-    for (int k = 0; k < PL; k++)
-        if (lane + 64 * k < D) o_s[wv][lane + 64 * k] = o[k];
-    if (lane == 0) l_s[wv] = l;
-    __syncthreads();
-    l = (l_s[0] + l_s[1]) + (l_s[2] + l_s[3]);
+    for (int k = LP; k < 64; k *= 2) {
+        l += __shfl_xor(l, k);
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] += __shfl_xor(o[e], k);
+    }
+    if constexpr (MANY) {
+        if (lane < LP) o_s[wv][lane] = o;
+        if (lane == 0) l_s[wv] = l;
+        __syncthreads();
+        if (threadIdx.x >= LP) return;
+        l = (l_s[0] + l_s[1]) + (l_s[2] + l_s[3]);
+        o = (o_s[0][lane] + o_s[1][lane]) + (o_s[2][lane] + o_s[3][lane]);
+    } else if (lane >= LP) {
+        return;
+    }
     float f = l == 0.0f ? 0.0f : 1.0f / l;
     if (a.gate) f *= 1.0f / (1.0f + expf(-a.gate[rh]));
-    if (threadIdx.x < D) {
-        const int d = threadIdx.x;
-        const float x = (o_s[0][d] + o_s[1][d]) + (o_s[2][d] + o_s[3][d]);
-        ((T*)a.out)[rh * D + d] = (T)(l == 0.0f ? 0.0f : x * f);
-    }
-    if (a.lse && threadIdx.x == 0) a.lse[rh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    uint2 w = {0u, 0u};
+    if (l != 0.0f) w = uint2{pack2<T>(o[0] * f, o[1] * f), pack2<T>(o[2] * f, o[3] * f)};
+    *(uint2*)((T*)a.out + rh * D + d) = w;
+    if (a.lse && d == 0) a.lse[rh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
-// column groups of 16 per workgroup: as many as the columns fill, up to what the registers hold
-int col_groups(int D, long long cols) {
-    const int most = D > 64 ? 2 : 4;
-    return cols <= 16 ? 1 : cols <= 32 || most == 2 ? 2 : 4;
-}
+// column groups of 16 a workgroup takes: one, or as many as the registers hold
+constexpr int many(int D) { return D > 64 ? 2 : 4; }
+int col_groups(int D, long long cols) { return cols <= 16 ? 1 : many(D); }
 
 long long shared_tiles(const pattn_args& a, int nt) { return ((long long)a.rows * a.grp + 16 * nt - 1) / (16 * nt); }
 long long own_tiles(const pattn_args& a, int nt, bool single) {
     return single ? (long long)a.n * ((a.grp + 16 * nt - 1) / (16 * nt)) : (long long)a.rows * a.grp / (16 * nt) + a.n;
 }
 
-template <class T, int D, int NT> hipError_t run_shared(const pattn_args& a, hipStream_t s) {
-    k_page_attn<T, D, NT, true><<<dim3((unsigned)(shared_tiles(a, NT) * a.n_kv * a.sp)), 256, 0, s>>>(a);
-    return hipGetLastError();
-}
-template <class T, int D, int NT> hipError_t run_own(const pattn_args& a, hipStream_t s) {
-    k_page_attn<T, D, NT, false><<<dim3((unsigned)(own_tiles(a, NT, !a.cu) * a.n_kv * a.so)), 256, 0, s>>>(a);
+template <class T, int D, int NTS, int NTO> hipError_t run_attn(const pattn_args& a, hipStream_t s) {
+    const long long blocks = NTS ? ((a.shared_blocks + 7ll) / 8 + (a.own_blocks + 7ll) / 8) * 8 : a.own_blocks;
+    k_page_attn<T, D, NTS, NTO><<<dim3((unsigned)blocks), 256, 0, s>>>(a);
     return hipGetLastError();
 }
 template <class T, int D> hipError_t run_all(const pattn_args& a, hipStream_t s) {
-    hipError_t e = hipSuccess;
-    if (a.sp) {
-        const int nt = col_groups(D, (long long)a.rows * a.grp);
-        if (nt == 1) e = run_shared<T, D, 1>(a, s);
-        else if (nt == 2) e = run_shared<T, D, 2>(a, s);
-        else if constexpr (D <= 64) e = run_shared<T, D, 4>(a, s);
-        if (e != hipSuccess) return e;
-    }
-    const int nt = col_groups(D, (long long)a.max_rows * a.grp);
-    if (nt == 1) e = run_own<T, D, 1>(a, s);
-    else if (nt == 2) e = run_own<T, D, 2>(a, s);
-    else if constexpr (D <= 64) e = run_own<T, D, 4>(a, s);
+    constexpr int M = many(D);
+    const int nts = a.sp ? col_groups(D, (long long)a.rows * a.grp) : 0, nto = col_groups(D, (long long)a.max_rows * a.grp);
+    hipError_t e;
+    if (nts == 0) e = nto == 1 ? run_attn<T, D, 0, 1>(a, s) : run_attn<T, D, 0, M>(a, s);
+    else if (nts == 1) e = run_attn<T, D, 1, 1>(a, s);   // (a request has no more columns than all of them)
+    else e = nto == 1 ? run_attn<T, D, M, 1>(a, s) : run_attn<T, D, M, M>(a, s);
     if (e != hipSuccess || a.sp + a.so == 1) return e;
-    k_page_join<T, D><<<dim3((unsigned)((long long)a.rows * a.n_head)), 256, 0, s>>>(a);
+    const long long rh = (long long)a.rows * a.n_head;
+    if (a.sp + a.so > 16) k_page_join<T, D, true><<<dim3((unsigned)rh), 256, 0, s>>>(a);
+    else k_page_join<T, D, false><<<dim3((unsigned)((rh + 3) / 4)), 256, 0, s>>>(a);
     return hipGetLastError();
 }
 template <class T> hipError_t run_dim(int D, const pattn_args& a, hipStream_t s) {
     return D == 32 ? run_all<T, 32>(a, s) : D == 64 ? run_all<T, 64>(a, s) : run_all<T, 128>(a, s);
 }
 
-void split(long long base, long long range, int* parts, int* chunk) {
-    long long p = 1024 / (base > 0 ? base : 1), most = (range + 255) / 256;
+void split(long long base, long long range, long long want, int* parts, int* chunk) {
+    long long p = want / (base > 0 ? base : 1), most = (range + 255) / 256;
     if (p > most) p = most;
     if (p < 1) p = 1;
     const long long c = ((range + p - 1) / p + 127) / 128 * 128;
@@ -473,27 +503,34 @@ void split(long long base, long long range, int* parts, int* chunk) {
 
 }  // namespace
 
-// Parts so that about four workgroups per compute unit run, of 256 keys or more.
+// Which workgroups take the shared positions, and into how many parts the keys go: about four workgroups per compute
+// unit, of 256 keys or more.
 bool page_attn_split(int D, bool single, pattn_args& a) {
+    const int nto = col_groups(D, (long long)a.max_rows * a.grp);
+    const long long own = own_tiles(a, nto, single), all = shared_tiles(a, col_groups(D, (long long)a.rows * a.grp));
+    a.own_at = (a.prefix_len + 31) / 32 * 32;
+    // Requests whose columns fill their workgroups read the shared positions themselves: sharing would not save reads,
+    // and nothing has to be joined. So do few requests with few shared positions
+    a.fused = a.prefix_len == 0 || own <= all * 2 || own * a.prefix_len <= 4096;
     a.sp = a.pchunk = 0;
     long long blocks = (long long)a.rows * a.n_head;
-    if (a.prefix_len) {
+    if (!a.fused) {
         const long long range = a.window && a.window + 31ll < a.prefix_len ? a.window + 31ll : a.prefix_len;
-        const long long base = shared_tiles(a, col_groups(D, (long long)a.rows * a.grp)) * a.n_kv;
-        split(base, range, &a.sp, &a.pchunk);
-        if (base * a.sp > blocks) blocks = base * a.sp;
+        split(all * a.n_kv, range, 512, &a.sp, &a.pchunk);
     }
-    const int nt = col_groups(D, (long long)a.max_rows * a.grp);
-    long long range = a.max_len;
+    long long range = (a.fused ? a.own_at : 0ll) + a.max_len;
     if (a.window) {
-        const long long rows = 16ll * nt / a.grp + 2, seen = a.window + 31ll + (rows < a.max_rows ? rows : a.max_rows);
+        const long long rows = 16ll * nto / a.grp + 2, seen = a.window + 63ll + (rows < a.max_rows ? rows : a.max_rows);
         if (seen < range) range = seen;
     }
-    const long long base = own_tiles(a, nt, single) * a.n_kv;
-    split(base, range, &a.so, &a.ochunk);
-    if (base * a.so > blocks) blocks = base * a.so;
+    split(own * a.n_kv, range, 1024, &a.so, &a.ochunk);
+    const long long shared_blocks = all * a.n_kv * a.sp, own_blocks = own * a.n_kv * a.so;
+    if (shared_blocks + own_blocks + 16 > blocks) blocks = shared_blocks + own_blocks + 16;
     // (columns of one kv head are counted in 32 bits in the kernel)
-    return blocks <= INT_MAX && (long long)a.rows * a.grp <= INT_MAX / 2;
+    if (blocks > INT_MAX || (long long)a.rows * a.grp > INT_MAX / 2) return false;
+    a.shared_blocks = (int)shared_blocks;
+    a.own_blocks = (int)own_blocks;
+    return true;
 }
 
 hipError_t launch_page_attn(int D, int type, const pattn_args& a, hipStream_t s) {

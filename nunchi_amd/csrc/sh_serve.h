@@ -40,8 +40,10 @@ struct pattn_args {
     const float* gate;
     void* out;
     float* lse;
-    // parts: the shared positions in sp parts of pchunk keys, each request's own in so parts of ochunk
-    int sp, so, pchunk, ochunk;
+    // parts: the shared positions in sp parts of pchunk keys (none: fused, each request reads them before its own), each
+    // request's own in so parts of ochunk; own ones are counted from own_at
+    int sp, so, pchunk, ochunk, own_at, shared_blocks, own_blocks;
+    bool fused;
     float* part_o;             // [sp + so][rows][n_head][D] sums of weights times values, not divided
     float2* part_ml;           // [sp + so][rows][n_head] maximum (powers of two) and sum of weights
 };
