@@ -11,12 +11,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libseoul_hip.so")
+MODULE = os.path.join(HERE, "_batch.so")     # the batch operators' CPython module (checks of tensors; links nothing)
 SOURCES = ["csrc/sh_kernels.hip", "csrc/sh_voice.hip", "csrc/sh_prefill.hip", "csrc/sh_noalloc.hip", "csrc/sh_codec.hip",
            "csrc/sh_ears.hip", "csrc/sh_calib.hip", "csrc/sh_pages.hip", "csrc/sh_page_attn.hip", "csrc/sh_sample.hip",
            "csrc/sh_engine.cpp", "csrc/sh_codec_host.cpp", "csrc/sh_ears_host.cpp", "csrc/sh_voice_host.cpp",
@@ -65,6 +67,16 @@ def build(verbose: bool = False) -> str:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("hipcc failed linking libseoul_hip.so")
         os.replace(tmp, LIB)
+        tmp = MODULE + f".tmp{os.getpid()}"
+        cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-I", sysconfig.get_paths()["include"], "-o", tmp,
+               os.path.join(HERE, "csrc", "py_batch.cpp")]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            sys.stderr.write(r.stdout + r.stderr)
+            raise RuntimeError("compiling _batch.so failed")
+        os.replace(tmp, MODULE)
     finally:
         shutil.rmtree(tmpdir, ignore_errors=True)
     return LIB

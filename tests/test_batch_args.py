@@ -90,8 +90,8 @@ def test_put_refused(bad):
 def test_attn_refused(bad):
     s = shape()
     size = C.c_size_t()
-    assert _lib().sh_page_attn_work(C.byref(s), 2, 2, 1, 40, 90, C.byref(size)) == 0 and size.value > 256
-    v = {**dict(ctx=BASE, shape=C.byref(s), n=2, rows=2, cu=None, max_rows=1, q=at(0), keys=at(1), values=at(2), prefix=at(3), prefix_len=40, table=at(4),
+    assert _lib().sh_page_attn_work(C.byref(s), 4, 4, 1, 4096, 90, C.byref(size)) == 0 and size.value > 256
+    v = {**dict(ctx=BASE, shape=C.byref(s), n=4, rows=4, cu=None, max_rows=1, q=at(0), keys=at(1), values=at(2), prefix=at(3), prefix_len=4096, table=at(4),
                 cols=8, len=at(5), max_len=90, gate=None, out=at(6), lse=None, work=at(7), bytes=size.value), **bad}
     assert _lib().sh_page_attn(*v.values()) == ARG
 

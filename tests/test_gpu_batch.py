@@ -500,11 +500,11 @@ def test_attn_leaves_rows_behind_and_past_max_rows(ctx):
     c = attn_case(20, [30, 12], 8, 2, 64, 16, "f16", prefix=20, add=[7, 3], extra_rows=5)
     check_attn(ctx, c)
     c = attn_case(20, [30, 12], 8, 2, 64, 16, "f16", prefix=20, add=[7, 3], extra_rows=5)
-    full = run_attn(ctx, c)[0].clone()
-    c["out"].fill_(7.0)
+    want, _, tol, _ = attn_reference(c)
     c["max_rows"] = 4
     out, _ = run_attn(ctx, c)
-    assert torch.equal(out[:4], full[:4]) and torch.equal(out[7:10], full[7:10])
+    rows = [0, 1, 2, 3, 7, 8, 9]
+    assert ((out.cpu().double()[rows] - want[rows]).abs() <= tol[rows]).all()
     assert (out[4:7] == 7).all() and (out[10:] == 7).all()
 
 
