@@ -185,6 +185,14 @@ int sh_step_batch(sh_ctx* ctx, sh_state* st, const int32_t* tokens, const float*
 int sh_generate(sh_ctx* ctx, sh_state* a, sh_state* b, int32_t first_a, int32_t first_b, int n_steps,
                 int32_t* out_a, int32_t* out_b, double* seconds);
 
+/* Sampled decode on the device: n_steps steps, each feeding back a word drawn from its word scores by sh_sample (below)
+ * with u_a[i] / u_b[i] as the random number of step i, for one (b null) or two conversations. The filters are the same
+ * for all steps: temp (0: the first maximum), top_k, top_p, min_p as there. Step i's word depends on the model, the words
+ * before it and u only; where nothing can be taken (all scores -inf or NaN) it is sh_generate's. */
+int sh_generate_sampled(sh_ctx* ctx, sh_state* a, sh_state* b, int32_t first_a, int32_t first_b, int n_steps, const double* u_a,
+                        const double* u_b, float temp, int32_t top_k, float top_p, float min_p, int32_t* out_a, int32_t* out_b,
+                        double* seconds);
+
 /* Every layer table read back to back with ncol (1 or 2) inputs riding each read, reps passes
  * (imi_seoul::bench_tables, seoul.cpp:657-685). ms_per_pass = best pass; avg_launch_us = mean GEMV launch
  * duration over all passes; bytes_per_pass = table bytes read per pass. */

@@ -20,7 +20,7 @@ LIB_PATH = os.path.join(HERE, "libseoul_hip.so")
 SH_OK, SH_E_ARG, SH_E_HIP, SH_E_FILE, SH_E_SHAPE, SH_E_CONTEXT_FULL, SH_E_STATE, SH_E_NOMEM = 0, -1, -2, -3, -4, -5, -6, -7
 EXPORTS = [
     "sh_last_error", "sh_create", "sh_create_on", "sh_destroy", "sh_load", "sh_info", "sh_check_model", "sh_state_new", "sh_state_free", "sh_state_reset",
-    "sh_state_pos", "sh_state_set_pos", "sh_step", "sh_step2", "sh_step_batch", "sh_generate", "sh_bench_tables",
+    "sh_state_pos", "sh_state_set_pos", "sh_step", "sh_step2", "sh_step_batch", "sh_generate", "sh_generate_sampled", "sh_bench_tables",
     "sh_bench_kernel", "sh_bench_step_kernel",
     "sh_q4_create", "sh_q4_free", "sh_q4_rows", "sh_q4_gemv", "sh_q4_gemm", "sh_q4_gemm_noalloc", "sh_q4_gemv_dev", "sh_q4_bench", "sh_q4_bench_kernel", "sh_q4_bench_graph",
     "sh_q4_gemv_group", "sh_q4_gemv_group_dev", "sh_q4_group_bench", "sh_expf", "sh_sync",
@@ -101,6 +101,7 @@ def load_library(path: str = LIB_PATH):
         "sh_step2": (i, [vp, vp, C.c_int32, vp, i, vp, C.c_int32, vp, i, vp, vp, vp, vp, vp, vp]),
         "sh_step_batch": (i, [vp, vp, vp, vp, i, i, vp, vp, vp, vp]),
         "sh_generate": (i, [vp, vp, vp, C.c_int32, C.c_int32, i, vp, vp, P(d)]),
+        "sh_generate_sampled": (i, [vp, vp, vp, C.c_int32, C.c_int32, i, vp, vp, f, C.c_int32, f, f, vp, vp, P(d)]),
         "sh_bench_tables": (i, [vp, i, i, P(d), P(d), P(d), P(i)]),
         "sh_bench_kernel": (i, [vp, i, i, i, P(d), P(d)]),
         "sh_bench_step_kernel": (i, [vp, i, i, i, P(d), P(d), P(i)]),
@@ -405,6 +406,25 @@ class Brain:
         secs = C.c_double(0)
         _check(_lib.sh_generate(self.ctx.h, a.h, b.h if b is not None else None, int(first), int(first_b), int(n),
                                 _p(oa), _p(ob), C.byref(secs)))
+        return (oa, ob, secs.value) if b is not None else (oa, secs.value)
+
+    def generate_sampled(self, first: int, u, temp: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
+                         b: State | None = None, first_b: int = 0, u_b=None, a: State | None = None):
+        """Sampled decode on the device (sh_generate_sampled): one step for each random number in u (and u_b). Returns ids
+        (and b's ids) and device seconds."""
+        a = a or self.state
+        u = np.ascontiguousarray(u, np.float64)
+        n = u.size
+        if b is not None:
+            u_b = np.ascontiguousarray(u_b, np.float64)
+            if u_b.size != n:
+                raise ValueError("u and u_b must hold as many random numbers")
+        oa = np.zeros(n, np.int32)
+        ob = np.zeros(n, np.int32) if b is not None else None
+        secs = C.c_double(0)
+        _check(_lib.sh_generate_sampled(self.ctx.h, a.h, b.h if b is not None else None, int(first), int(first_b), int(n), _p(u),
+                                        _p(u_b) if b is not None else None, float(temp), int(top_k), float(top_p), float(min_p), _p(oa), _p(ob),
+                                        C.byref(secs)))
         return (oa, ob, secs.value) if b is not None else (oa, secs.value)
 
     def bench_tables(self, ncol: int = 1, reps: int = 10):

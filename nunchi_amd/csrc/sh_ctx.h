@@ -104,6 +104,8 @@ struct sh_ctx {
     int* part_i = nullptr;
     int32_t* gen_out = nullptr;       // device-side greedy ids [2][gen_cap]
     int gen_cap = 0;
+    char* gen_pick = nullptr;         // sampled decode: random numbers [steps][conversations], the picks and the filters
+    size_t gen_pick_cap = 0;
     float* bench_x = nullptr;         // kernel-API input/output staging
     float* bench_y = nullptr;
     size_t bench_cap = 0;

@@ -11,11 +11,13 @@
 #include <cstdlib>
 #include <cstring>
 #include <memory>
+#include <new>
 #include <string>
 #include <vector>
 
 #include "gguf_file.h"
 #include "sh_ctx.h"
+#include "sh_serve.h"
 
 using namespace sh;
 
@@ -504,6 +506,7 @@ int sh_destroy(sh_ctx* c) {
     if (c->P_dev) (void)hipFree(c->P_dev);
     if (c->P_host) (void)hipHostFree(c->P_host);
     if (c->gen_out) (void)hipFree(c->gen_out);
+    if (c->gen_pick) (void)hipFree(c->gen_pick);
     if (c->ev0) (void)hipEventDestroy(c->ev0);
     if (c->ev1) (void)hipEventDestroy(c->ev1);
     if (c->stream && c->own_stream) (void)hipStreamDestroy(c->stream);
@@ -949,6 +952,88 @@ int sh_generate(sh_ctx* c, sh_state* a, sh_state* b, int32_t fa, int32_t fb, int
     for (int i = 0; i < n; i++) {
         if (g) HIPCHK(hipGraphLaunch(g, c->stream));
         else if ((rc = enqueue_step(c, M, true)) != SH_OK) return rc;
+    }
+    HIPCHK(hipEventRecord(c->ev1, c->stream));
+    if (out_a) HIPCHK(hipMemcpyAsync(out_a, c->gen_out, sizeof(int32_t) * n, hipMemcpyDeviceToHost, c->stream));
+    if (out_b && b) HIPCHK(hipMemcpyAsync(out_b, c->gen_out + c->gen_cap, sizeof(int32_t) * n, hipMemcpyDeviceToHost, c->stream));
+    HIPCHK(hipStreamSynchronize(c->stream));
+    float ms = 0.0f;
+    HIPCHK(hipEventElapsedTime(&ms, c->ev0, c->ev1));
+    if (seconds) *seconds = ms * 1e-3;
+    for (int m = 0; m < M; m++) st[m]->pos += n;
+    return SH_OK;
+}
+
+int sh_generate_sampled(sh_ctx* c, sh_state* a, sh_state* b, int32_t fa, int32_t fb, int n, const double* ua, const double* ub, float temp,
+                        int32_t top_k, float top_p, float min_p, int32_t* out_a, int32_t* out_b, double* seconds) {
+    if (!c || !c->loaded) return fail(SH_E_STATE, "sh_generate_sampled: no model loaded");
+    if (!a || n < 0 || (b && b == a)) return fail(SH_E_ARG, "sh_generate_sampled: bad argument");
+    if (n && (!ua || (b && !ub))) return fail(SH_E_ARG, "sh_generate_sampled: random numbers missing");
+    if (!(temp >= 0.0f)) return fail(SH_E_ARG, "sh_generate_sampled: temp is negative or NaN");
+    const int M = b ? 2 : 1, V = c->info.n_vocab;
+    if (V > SAMPLE_MAX_VOCAB) return fail(SH_E_SHAPE, "sh_generate_sampled: more than 524288 words");
+    sh_state* st[2] = {a, b};
+    const int32_t first[2] = {fa, fb};
+    for (int m = 0; m < M; m++) {
+        if (st[m]->ctx != c) return fail(SH_E_STATE, "sh_generate_sampled: state belongs to another context");
+        if (first[m] < 0 || first[m] >= V) return fail(SH_E_ARG, "sh_generate_sampled: first token out of range");
+        if (st[m]->pos + (long long)n > c->info.n_ctx) {
+            fprintf(stderr, "seoul-hip: context full (%d)\n", c->info.n_ctx);
+            return fail(SH_E_CONTEXT_FULL, "sh_generate_sampled: context full");
+        }
+    }
+    HIPCHK(hipSetDevice(c->device));
+    if (n > c->gen_cap) {
+        HIPCHK(regrow((void**)&c->gen_out, sizeof(int32_t) * 2 * (size_t)n));
+        c->gen_cap = n;
+    }
+    // on the device: the filters (one of each a conversation), the picks, the random numbers step by step
+    struct filters { float temp[2], top_p[2], min_p[2]; int32_t top_k[2], ids[2], unused[2]; };
+    static_assert(sizeof(filters) % sizeof(double) == 0, "the random numbers follow");
+    const size_t bytes = sizeof(filters) + (size_t)n * M * sizeof(double);
+    std::unique_ptr<char[]> host(new (std::nothrow) char[bytes]);
+    if (!host) return fail(SH_E_NOMEM, "sh_generate_sampled: out of memory");
+    if (bytes > c->gen_pick_cap) {
+        HIPCHK(regrow((void**)&c->gen_pick, bytes));
+        c->gen_pick_cap = bytes;
+    }
+    filters f{{temp, temp}, {top_p, top_p}, {min_p, min_p}, {top_k, top_k}, {-1, -1}, {0, 0}};
+    memcpy(host.get(), &f, sizeof f);
+    double* u = reinterpret_cast<double*>(host.get() + sizeof f);
+    for (int i = 0; i < n; i++) {
+        u[(size_t)i * M] = ua[i];
+        if (b) u[(size_t)i * M + 1] = ub[i];
+    }
+    hipGraphExec_t g;
+    int rc = get_graph(c, M, true, &g);
+    if (rc != SH_OK) return rc;
+    step_params& P = *c->P_host;
+    memset(&P, 0, sizeof P);
+    for (int m = 0; m < M; m++) {
+        P.token[m] = first[m];
+        fill_state(P, m, st[m]);
+    }
+    HIPCHK(hipMemcpyAsync(c->gen_pick, host.get(), bytes, hipMemcpyHostToDevice, c->stream));
+    HIPCHK(hipMemcpyAsync(c->P_dev, &P, sizeof P, hipMemcpyHostToDevice, c->stream));
+    HIPCHK(hipEventRecord(c->ev0, c->stream));
+    filters* fd = reinterpret_cast<filters*>(c->gen_pick);
+    sample_args s{};
+    s.rows = M;
+    s.vocab = V;
+    s.type = TY_F32;
+    s.ld = V;
+    s.scores = c->logits;
+    s.temp = fd->temp;
+    s.top_k = fd->top_k;
+    s.top_p = fd->top_p;
+    s.min_p = fd->min_p;
+    s.ids = fd->ids;
+    for (int i = 0; i < n; i++) {
+        if (g) HIPCHK(hipGraphLaunch(g, c->stream));
+        else if ((rc = enqueue_step(c, M, true)) != SH_OK) return rc;
+        s.u = reinterpret_cast<const double*>(c->gen_pick + sizeof(filters)) + (size_t)i * M;
+        HIPCHK(launch_sample(s, c->stream));
+        HIPCHK(launch_take(M, fd->ids, c->P_dev->best, c->P_dev->token, c->gen_out + i, c->gen_cap, c->stream));
     }
     HIPCHK(hipEventRecord(c->ev1, c->stream));
     if (out_a) HIPCHK(hipMemcpyAsync(out_a, c->gen_out, sizeof(int32_t) * n, hipMemcpyDeviceToHost, c->stream));

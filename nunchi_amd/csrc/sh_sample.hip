@@ -789,7 +789,20 @@ template <class T> hipError_t run(const sample_args& a, hipStream_t s) {
     return words <= 1024 * 32 ? run_held<T, 1024, 1>(a, s) : words <= HELD_WORDS ? run_held<T, 512, 6>(a, s) : run_held<T, 1024, 0>(a, s);
 }
 
+__global__ void k_take(int n, const int32_t* ids, const int32_t* fallback, int32_t* token, int32_t* out, int ld) {
+    const int m = threadIdx.x;
+    if (m >= n) return;
+    const int id = ids[m] < 0 ? fallback[m] : ids[m];
+    token[m] = id;
+    out[(size_t)m * ld] = id;
+}
+
 }  // namespace
+
+hipError_t launch_take(int n, const int32_t* ids, const int32_t* fallback, int32_t* token, int32_t* out, int ld, hipStream_t s) {
+    k_take<<<1, 64, 0, s>>>(n, ids, fallback, token, out, ld);
+    return hipGetLastError();
+}
 
 hipError_t launch_sample(const sample_args& a, hipStream_t s) {
     return a.type == TY_F32 ? run<float>(a, s) : a.type == TY_F16 ? run<_Float16>(a, s) : run<__bf16>(a, s);

@@ -67,5 +67,7 @@ hipError_t launch_page_put(int D, int src_type, int type, const put_args& a, hip
 bool page_attn_split(int D, bool single, pattn_args& a);
 hipError_t launch_page_attn(int D, int type, const pattn_args& a, hipStream_t s);
 hipError_t launch_sample(const sample_args& a, hipStream_t s);
+// the words of ids[n] (a word < 0: fallback's) to token[n] and, for conversation m, out[m * ld]
+hipError_t launch_take(int n, const int32_t* ids, const int32_t* fallback, int32_t* token, int32_t* out, int ld, hipStream_t s);
 
 }  // namespace sh

@@ -747,6 +747,48 @@ def test_engine_on_the_default_stream(tiny_model):
         assert np.array_equal(a.generate(5, 6)[0], b.generate(5, 6)[0])
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(temp=0.7, top_k=20), dict(top_p=0.8, temp=1.3), dict(min_p=0.1), dict(temp=0.0)], ids=str)
+def test_generate_sampled(mid_model, kw):
+    """The device loop against single steps whose word scores go through the reference: one conversation and two."""
+    rng = np.random.default_rng(8)
+    brain = nunchi_amd.Brain(mid_model, n_ctx=64)
+    u, ub = rng.uniform(size=9), rng.uniform(size=9)
+    f32 = {k: (np.float32(v).item() if k != "top_k" else v) for k, v in kw.items()}
+
+    def steps(first, u, st):
+        tok, out = first, []
+        for x in u:
+            _, scores, _ = brain.step(tok, st=st)
+            tok = sample_reference(scores, x, **f32)[0]
+            out.append(tok)
+        return out
+
+    ids, secs = brain.generate_sampled(7, u, **kw)
+    assert secs > 0 and brain.pos == 9
+    assert ids.tolist() == steps(7, u, brain.new_state())
+    if kw.get("temp") == 0.0:
+        assert ids.tolist() == brain.generate(7, 9, a=brain.new_state())[0].tolist()
+    a, b = brain.new_state(), brain.new_state()
+    ia, ib, _ = brain.generate_sampled(11, u, b=b, first_b=12, u_b=ub, a=a, **kw)
+    assert ia.tolist() == steps(11, u, brain.new_state()) and ib.tolist() == steps(12, ub, brain.new_state())
+    assert a.pos == b.pos == 9
+
+
+def test_generate_sampled_refuses(tiny_model):
+    brain = nunchi_amd.Brain(tiny_model, n_ctx=16)
+    for bad in (dict(temp=-1.0), dict(temp=float("nan")), dict(first=-1), dict(first=1000)):
+        kw = {"first": 3, "u": [0.5] * 4, **bad}
+        with pytest.raises(nunchi_amd.SeoulError):
+            brain.generate_sampled(**kw)
+    with pytest.raises(nunchi_amd.ContextFull):
+        brain.generate_sampled(3, [0.5] * 17)
+    with pytest.raises(nunchi_amd.SeoulError):
+        brain.generate_sampled(3, [0.5], b=brain.state, u_b=[0.5])
+    with pytest.raises(ValueError):
+        brain.generate_sampled(3, [0.5], b=brain.new_state(), u_b=[0.5, 0.5])
+    assert brain.pos == 0 and brain.generate_sampled(3, [])[0].size == 0
+
+
 class Serving:
     """A small serving loop: conversations behind a shared prefix, step by step, in pages."""
 
