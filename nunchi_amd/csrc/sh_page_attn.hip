@@ -18,12 +18,14 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 template <class T> struct mat;
 template <> struct mat<_Float16> {
     static constexpr unsigned EXP = 0x7C00u;   // the exponent bits of one value: all set in infinities and NaN
+    static constexpr float SLACK = 4.0f, LIFT = 11.0f;   // weights up to 2^15; their last place is 2^-35 of the largest
     static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
 };
 template <> struct mat<__bf16> {
     static constexpr unsigned EXP = 0x7F80u;
+    static constexpr float SLACK = 8.0f, LIFT = 0.0f;    // (eight bits of exponent hold any weight)
     static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
@@ -71,8 +73,10 @@ template <int D, int NT> struct join_space {
 // eight scores are eight neighbouring keys, which are its operand of the second product (O^T = V^T P^T) as they are.
 // V's operand is eight keys of one dimension: each lane loads the same D / 16 dimensions of eight keys and turns the
 // block with byte permutes. Nothing passes through LDS before the waves are joined. Weights are rounded to the values'
-// 16 bits for the second product, relative to a maximum that is at most 2^8 behind the true one (the accumulators are
-// rescaled only when a score passes it by more): their sum stays in 32 bits.
+// 16 bits for the second product, as the matrix units take them; their sum stays in 32 bits. They are relative to a
+// maximum that is up to 2^SLACK behind the true one (the accumulators are rescaled only when a score passes it by more)
+// and 2^LIFT below it: with f16's five bits of exponent, weights below 2^-25 of the largest would all be lost, and a
+// hundred thousand of them are a part of the sum that shows.
 // SHARED: the columns of all requests over the shared positions. Else one request's columns over its own positions, and
 // over the shared ones before them where no SHARED part takes them (a.fused).
 template <class T, int D, int NT, bool SHARED>
@@ -127,10 +131,10 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, joi
             const int k = !SHARED ? i : a.cu ? request_of(a.cu, a.n, row[t]) : row[t];
             const int first_row = a.cu ? a.cu[k] : k, rows_k = a.cu ? a.cu[k + 1] - first_row : 1;
             // (at most its last place: row starts that contradict each other lead nowhere else)
-            at = (int)min(min(max(a.len[k], 0), own_max) - (long long)rows_k + (row[t] - first_row), own_max - 1ll);
+            at = (int)max(min(min(max(a.len[k], 0), own_max) - (long long)rows_k + (row[t] - first_row), own_max - 1ll), -1ll - a.rows);
         }
         // the first position of the line that a window leaves
-        const int from = a.window ? L0 + at + 1 - a.window : 0;
+        const int from = a.window ? (int)max(L0 + at + 1ll - a.window, 0ll) : 0;
         if constexpr (SHARED) {
             lo[t] = min(max(from, 0), L0);
             hi[t] = L0;
@@ -233,10 +237,10 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, joi
                 float top = x[0];          // (NaN is passed over)
 #pragma unroll
                 for (int k = 1; k < 8; k++) top = fmaxf(top, x[k]);
-                if (__any(top > m[t] + 8.0f)) {
+                if (__any(top > m[t] + (mat<T>::SLACK + mat<T>::LIFT))) {
                     top = fmaxf(top, __shfl_xor(top, 16));
                     top = fmaxf(top, __shfl_xor(top, 32));
-                    const float to = fmaxf(m[t], top), f = rescale(m[t], to);
+                    const float to = fmaxf(m[t], top - mat<T>::LIFT), f = rescale(m[t], to);
                     l[t] *= f;
 #pragma unroll
                     for (int e = 0; e < E; e++) o[e][t] *= f;

@@ -335,7 +335,8 @@ def attn_reference(c):
             tol_lse[r] = off + 2.0 ** -23 * lse[r].abs()
             h = HALF[c["kind"]]
             big = v.abs().amax(0).amax(-1)
-            under = 2.0 ** -25 * len(seen) if c["kind"] == "f16" else 0.0
+            # (f16 weights are 2^11 of the running maximum's: below 2^-14 their places are 2^-24 apart)
+            under = 2.0 ** -36 * len(seen) if c["kind"] == "f16" else 0.0
             tol[r, :, 0] = (h * 1.01 + under + 2 * off) * big
         r0 += c["counts"][i]
     if c["gate"] is not None:
@@ -409,6 +410,32 @@ def test_attn_finds_one_key_anywhere(ctx, kind):
         assert ((out[0].float() - want).abs() <= 2 * HALF[kind] * want.abs() + 2.0 ** -25 + 2200 * math.exp(-30) * 6).all(), p
         assert abs(lse[0, 0].item() - 30.0) < 1e-5
         c["keys"][pid, 0, o, 0] = 0.0
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_attn_many_small_weights(ctx, kind):
+    """20000 keys of weights 2^-25.5 of the largest, whose value is 0: the output is the small ones' sum. Each weight is
+    rounded by half a step (h, or 2^-25 below 2^-14 in f16: here 2^-25.5 + 11), the result by h."""
+    N, n, page = 20000, 512, 16
+    pages = N // page
+    keys, values = torch.zeros(pages, 2, page, 64, dtype=TYPES[kind], device="cuda"), torch.ones(pages, 2, page, 64, dtype=TYPES[kind], device="cuda")
+    q = torch.zeros(n, 2, 64, dtype=TYPES[kind], device="cuda")
+    q[..., 0] = 1
+    keys[700, :, 5, 0] = 17.625
+    values[700, :, 5] = 0
+    shape = nunchi_amd.PageShape(2, 2, 64, page, pages, dtype=kind, scale=1.0)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(n, 1)       # (all requests read the same pages)
+    out, work = torch.empty_like(q), torch.empty(nunchi_amd.page_attn_work(shape, n, n, N), dtype=torch.uint8, device="cuda")
+    nunchi_amd.page_attn(ctx, shape, q, keys, values, table, i32([N] * n), out, work, N)
+    e = math.exp(-keys[700, 0, 5, 0].item())
+    want = (N - 1) * e / (1 + (N - 1) * e)
+    assert ((out.double() / want - 1).abs() <= 2 * HALF[kind] + 2.0 ** -25 / 2.0 ** -14.5 + 2.0 ** -19).all(), out.double().mean().item() / want
+
+
+def test_attn_windows_of_any_length(ctx):
+    """A window that passes every position leaves nothing out, also for rows whose request holds less than them."""
+    for window in (2 ** 31 - 1, 2 ** 31 - 200, 290, 291):
+        check_attn(ctx, attn_case(21, [0, 200], 8, 2, 64, 16, "f16", prefix=90, add=[200, 30], window=window))
 
 
 def test_attn_large_scores(ctx):
