@@ -329,7 +329,8 @@ int sh_voice_sample(sh_voice* v, const int32_t* hist, int n_frames, const double
  * 21-26), and picks greedily (imi/core/hear.cpp:66-72). All pointers are device memory on the context's device; calls are
  * enqueued on the context's stream without waiting (sh_sync waits), allocate nothing and may be captured into a graph.
  * Lengths, tables and slots live on the device, so what they hold is checked there: an entry that points outside its
- * array is treated as said below and never followed. Arrays of 16-bit types, keys and values start on 16 bytes.
+ * array is treated as said below and never followed. Arrays of 16-bit types, keys and values start on 16 bytes. An output that
+ * overlaps an input or another output is refused (SH_E_ARG).
  *
  * A cache is keys and values in pages of `page` positions, for one layer: [n_pages][n_kv][page][head_dim] each. A slot is
  * a place for one position: page id * page + position in the page. Types as in sh_tensor: SH_F32, SH_F16, SH_BF16. */
@@ -357,7 +358,7 @@ typedef struct {
  *   taken_out  [1]        pages given out after the step
  * A request is refused (slots -1, no pages) when a length is negative, its pages pass `cols`, its rows pass `rows`, or
  * free_pages has not enough left for it and those before it. Entries of slots and pos behind the last request's rows stay
- * as they were. n up to 4096. No output may overlap an input (SH_E_ARG). */
+ * as they were. n up to 4096. */
 int sh_page_plan(sh_ctx* ctx, int n, const int32_t* held, const int32_t* add, int page, int32_t* table, int cols,
                  const int32_t* free_pages, int n_free, const int32_t* taken, int32_t* taken_out, int32_t* len,
                  int32_t* cu, int64_t* slots, int32_t* pos, int rows, int pos0);
@@ -380,7 +381,9 @@ int sh_page_put(sh_ctx* ctx, const sh_page_shape* shape, int rows, const void* q
  * these the shape's window. out[r][h] = sum of softmax(scale q k) v, times sigmoid(gate[r][h]) where gate [rows][n_head]
  * is given (imi/core/seoul.cpp:433-453); lse [rows][n_head] (null: none) gets the logarithm of the sum of e^score, before
  * the gate. A row that sees nothing gives zeros and -inf. Keys of a page id outside [0, n_pages) count as not there. Rows
- * behind the last request's, and those past max_rows of their request, stay as they were.
+ * behind the last request's, and those past max_rows of their request, stay as they were. Weights are rounded to the
+ * shape's type for their products with the values, sums are 32 bits: out is within half a place of the largest value seen
+ * (and, where a single key outweighs a million others by 2^30, another quarter of one in f16).
  * The shared positions are read once for the whole batch, as one matrix product for all rows. work: sh_page_attn_work's
  * bytes for the same sizes, on 256 bytes, the call's own until it is done (calls that may run at once, captured graphs
  * among them, need one each; nothing is kept in it between calls). */

@@ -79,7 +79,8 @@ __global__ __launch_bounds__(PLAN_T) void k_page_plan(plan_args a) {
     }
     if (t == PLAN_T - 1) { cu_s[a.n] = sat(r_at); st_s[a.n] = sat(p_at); }
     __syncthreads();
-    const int taken = max(a.taken[0], 0), total = min(cu_s[a.n], a.rows), opened = st_s[a.n];
+    const int taken = max(a.taken[0], 0), total = min(cu_s[a.n], a.rows);
+    const int opened = min(st_s[a.n], max(a.n_free - taken, 0));   // (what lies behind fits no request)
     auto fits = [&](const plan_req& q, int i) {
         return q.ok && cu_s[i + 1] <= a.rows && cu_s[i + 1] < INT_MAX && (q.need == 0 || (long long)taken + st_s[i + 1] <= a.n_free);
     };

@@ -40,6 +40,18 @@ bool meet(const void* p, size_t np, const void* q, size_t nq) {
     return np && nq && a < b + nq && b < a + np;
 }
 
+struct extent { const void* p; size_t n; };
+// null when no output overlaps an input or another output
+template <size_t I, size_t O> const char* overlap(const extent (&in)[I], const extent (&out)[O]) {
+    for (size_t i = 0; i < O; i++) {
+        for (auto& x : in)
+            if (out[i].p && x.p && meet(out[i].p, out[i].n, x.p, x.n)) return "an output overlaps an input";
+        for (size_t j = 0; j < i; j++)
+            if (out[i].p && out[j].p && meet(out[i].p, out[i].n, out[j].p, out[j].n)) return "two outputs overlap";
+    }
+    return nullptr;
+}
+
 int page_log(int page) {
     for (int l = 4; l <= 8; l++)
         if (page == 1 << l) return l;
@@ -73,7 +85,7 @@ const char* attn_sizes(const sh_page_shape* s, int n, int rows, int max_rows, in
     a.n_kv = s->n_kv;
     a.grp = s->n_head / s->n_kv;
     a.page_log = page_log(s->page);
-    a.window = s->window;
+    a.window = s->window < prefix_len + max_len ? s->window : 0;   // (a longer one leaves nothing out)
     a.max_rows = max_rows < rows ? max_rows : rows > 0 ? rows : 1;
     a.prefix_len = prefix_len;
     a.max_len = max_len;
@@ -113,14 +125,9 @@ int sh_page_plan(sh_ctx* c, int n, const int32_t* held, const int32_t* add, int 
     if (cols < 0 || n_free < 0 || rows < 0 || pos0 < 0) return bad(who, "a size is negative");
     if ((cols && !table) || (n_free && !free_pages) || (rows && (!slots || !pos))) return bad(who, "null");
     const size_t in4 = (size_t)n * 4;
-    struct { const void* p; size_t n; } in[4] = {{held, in4}, {add, in4}, {free_pages, (size_t)n_free * 4}, {taken, 4}},
-        out[6] = {{table, (size_t)n * cols * 4}, {taken_out, 4}, {len, in4}, {cu, in4 + 4}, {slots, (size_t)rows * 8}, {pos, (size_t)rows * 4}};
-    for (int i = 0; i < 6; i++) {
-        for (auto& x : in)
-            if (meet(out[i].p, out[i].n, x.p, x.n)) return bad(who, "an output overlaps an input");
-        for (int j = 0; j < i; j++)
-            if (meet(out[i].p, out[i].n, out[j].p, out[j].n)) return bad(who, "two outputs overlap");
-    }
+    const extent in[] = {{held, in4}, {add, in4}, {free_pages, (size_t)n_free * 4}, {taken, 4}},
+                 out[] = {{table, (size_t)n * cols * 4}, {taken_out, 4}, {len, in4}, {cu, in4 + 4}, {slots, (size_t)rows * 8}, {pos, (size_t)rows * 4}};
+    if (const char* f = overlap(in, out)) return bad(who, f);
     const on_device dev(c->device);
     if (dev.e != hipSuccess) return done(dev.e, who);
     plan_args a{};
@@ -160,6 +167,11 @@ int sh_page_put(sh_ctx* c, const sh_page_shape* s, int rows, const void* qkv, lo
     if ((rows * heads + 15) / 16 > INT_MAX) return bad(who, "more rows than one launch holds");
     if (off(qkv, src_type == SH_F32 ? 4 : 2)) return bad(who, "qkv is not aligned to its type");
     if (off(q_out, 16) || off(keys, 16) || off(values, 16)) return bad(who, "queries, keys and values start on 16 bytes");
+    const size_t cache = (size_t)s->n_pages * s->n_kv * s->page * s->head_dim * 2, vec = (size_t)s->head_dim * 4;
+    const extent in[] = {{qkv, ((size_t)(rows - 1) * ld + heads * s->head_dim) * (src_type == SH_F32 ? 4 : 2)}, {slots, (size_t)rows * 8}, {pos, (size_t)rows * 4},
+                         {q_norm, vec}, {k_norm, vec}, {rope, rope ? (size_t)n_rope * vec : 0}},
+                 out[] = {{q_out, (size_t)rows * s->n_head * s->head_dim * 2}, {keys, cache}, {values, cache}};
+    if (const char* f = overlap(in, out)) return bad(who, f);
     const on_device dev(c->device);
     if (dev.e != hipSuccess) return done(dev.e, who);
     put_args a{};
@@ -216,6 +228,12 @@ int sh_page_attn(sh_ctx* c, const sh_page_shape* s, int n, int rows, const int32
     size_t sums, all;
     attn_work(a, s->head_dim, &sums, &all);
     if (all && (!work || work_bytes < all || off(work, 256))) return bad(who, "work is missing, smaller than sh_page_attn_work says, or not on 256 bytes");
+    const size_t q_bytes = (size_t)rows * s->n_head * s->head_dim * 2, rh = (size_t)rows * s->n_head * sizeof(float),
+                 cache = (size_t)s->n_pages * s->n_kv * s->page * s->head_dim * 2;
+    const extent in[] = {{q, q_bytes}, {keys, cache}, {values, cache}, {gate, rh}, {len, (size_t)n * 4}, {table, (size_t)n * cols * 4}, {cu, ((size_t)n + 1) * 4},
+                         {prefix, ((size_t)prefix_len + s->page - 1) / s->page * 4}},
+                 to[] = {{out, q_bytes}, {lse, rh}, {work, all}};
+    if (const char* f = overlap(in, to)) return bad(who, f);
     const on_device dev(c->device);
     if (dev.e != hipSuccess) return done(dev.e, who);
     a.cols = cols;
@@ -258,6 +276,10 @@ int sh_sample(sh_ctx* c, int rows, int vocab, const void* scores, long long ld, 
     if (ld < vocab) return bad(who, "a row (ld) is shorter than vocab");
     if (off(scores, type == SH_F32 ? 4 : 2)) return bad(who, "scores are not aligned to their type");
     if (!work || work_bytes < need || off(work, 256)) return bad(who, "work is missing, smaller than sh_sample_work says, or not on 256 bytes");
+    const size_t each = (size_t)rows * 4;
+    const extent in[] = {{scores, ((size_t)(rows - 1) * ld + vocab) * (type == SH_F32 ? 4 : 2)}, {temp, each}, {top_k, each}, {top_p, each}, {min_p, each}, {u, each * 2}},
+                 out[] = {{ids, each}, {chance, each}};
+    if (const char* f = overlap(in, out)) return bad(who, f);
     const on_device dev(c->device);
     if (dev.e != hipSuccess) return done(dev.e, who);
     sample_args a{};

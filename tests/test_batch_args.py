@@ -75,7 +75,10 @@ def test_plan_refused(bad):
 
 @pytest.mark.parametrize("bad", [dict(ctx=None), dict(rows=-1), dict(qkv=None), dict(qkv=at(0) + 2), dict(ld=767), dict(src=2), dict(src=8), dict(rope=at(4)),
                                  dict(rope=at(4), pos=at(5), n_rope=0), dict(slots=None), dict(q=at(6) + 8), dict(keys=None), dict(keys=at(1) + 2),
-                                 dict(values=None), dict(values=at(2) + 4), dict(rows=(1 << 31) - 1, ld=1 << 40)], ids=str)
+                                 dict(values=None), dict(values=at(2) + 4), dict(rows=(1 << 31) - 1, ld=1 << 40),
+                                 # an output over an input, or over another output
+                                 dict(q=at(0)), dict(q=at(0) + (2 * 768 + 767) * 4 // 16 * 16), dict(keys=at(0) + 16), dict(values=at(3)), dict(keys=at(2) + 16),
+                                 dict(q=at(1) + 10 * 2 * 16 * 64 * 2 - 16), dict(q=at(2))], ids=str)
 def test_put_refused(bad):
     s = shape(n_head=8, n_kv=2) if "ld" not in bad or bad["ld"] < 1 << 20 else shape(n_head=65536, n_kv=1)
     v = {**dict(ctx=BASE, shape=C.byref(s), rows=3, qkv=at(0), ld=768, src=0, q_norm=None, k_norm=None, rope=None, n_rope=5, pos=None, slots=at(3),
@@ -86,7 +89,10 @@ def test_put_refused(bad):
 @pytest.mark.parametrize("bad", [dict(ctx=None), dict(n=0), dict(rows=-1), dict(rows=3), dict(max_rows=2), dict(max_rows=0, cu=at(9)), dict(q=None), dict(q=at(0) + 8),
                                  dict(keys=None), dict(keys=at(1) + 2), dict(values=None), dict(values=at(2) + 8), dict(prefix=None), dict(prefix_len=-1),
                                  dict(prefix_len=(1 << 31) - 1), dict(table=None), dict(cols=-1), dict(len=None), dict(max_len=-1), dict(out=None),
-                                 dict(out=at(6) + 2), dict(work=None), dict(work=at(7) + 64), dict(bytes=100)], ids=str)
+                                 dict(out=at(6) + 2), dict(work=None), dict(work=at(7) + 64), dict(bytes=100),
+                                 # an output over an input, or over another output
+                                 dict(out=at(0)), dict(out=at(1) + 64), dict(out=at(2)), dict(work=at(5)), dict(lse=at(6)), dict(lse=at(0) + 32), dict(lse=at(7) + 256),
+                                 dict(gate=at(6) + 16), dict(out=at(3)), dict(out=at(4) + 112), dict(cu=at(7))], ids=str)
 def test_attn_refused(bad):
     s = shape()
     size = C.c_size_t()
@@ -113,7 +119,8 @@ def test_attn_work_fits_every_split(n, rows, max_rows, prefix, own):
 
 
 @pytest.mark.parametrize("bad", [dict(ctx=None), dict(rows=-1), dict(vocab=0), dict(vocab=524289), dict(scores=None), dict(ld=99), dict(type=3), dict(u=None),
-                                 dict(ids=None), dict(scores=at(0) + 2), dict(work=None), dict(work=at(3) + 128), dict(bytes=16)], ids=str)
+                                 dict(ids=None), dict(scores=at(0) + 2), dict(work=None), dict(work=at(3) + 128), dict(bytes=16),
+                                 dict(ids=at(0) + 64), dict(chance=at(0)), dict(chance=at(2) + 4), dict(ids=at(1) + 8)], ids=str)
 def test_sample_refused(bad):
     size = C.c_size_t()
     assert _lib().sh_sample_work(2, 100, C.byref(size)) == 0
