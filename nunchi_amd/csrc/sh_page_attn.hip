@@ -224,7 +224,7 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, joi
 #pragma unroll
                     for (int c = 0; c < CH; c++) s = mat<T>::mul(kf[b][c], qf[c][t], s);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) x[4 * b + r] = s[r] * a.c;
+                    for (int r = 0; r < 4; r++) x[4 * b + r] = s[r];
                 }
                 if (!full) {
                     const int stop = min(hi[t], end);
@@ -237,6 +237,7 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, joi
                 float top = x[0];          // (NaN is passed over)
 #pragma unroll
                 for (int k = 1; k < 8; k++) top = fmaxf(top, x[k]);
+                top *= a.c;
                 if (__any(top > m[t] + (mat<T>::SLACK + mat<T>::LIFT))) {
                     top = fmaxf(top, __shfl_xor(top, 16));
                     top = fmaxf(top, __shfl_xor(top, 32));
@@ -250,7 +251,7 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, joi
                 float sum = 0.0f;
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
-                    x[k] = exp2_(x[k] - ref);
+                    x[k] = exp2_(fmaf(x[k], a.c, -ref));
                     sum += x[k];
                 }
                 l[t] += sum;

@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <string>
@@ -90,7 +91,7 @@ const char* attn_sizes(const sh_page_shape* s, int n, int rows, int max_rows, in
     a.prefix_len = prefix_len;
     a.max_len = max_len;
     a.n_pages = (int)s->n_pages;
-    a.c = (s->scale > 0.0f ? s->scale : 1.0f / std::sqrt((float)s->head_dim)) * 1.44269504f;
+    a.c = std::fmax((s->scale > 0.0f ? s->scale : 1.0f / std::sqrt((float)s->head_dim)) * 1.44269504f, FLT_MIN);   // (0 times a masked -inf is NaN)
     if (!page_attn_split(s->head_dim, single, a)) return "more workgroups than one launch holds: fewer rows at once";
     return nullptr;
 }

@@ -449,6 +449,7 @@ def test_attn_large_scores(ctx):
 
 def test_attn_scale_and_no_gate(ctx):
     check_attn(ctx, attn_case(12, [50, 9], 8, 2, 64, 16, "f16", prefix=20, scale=0.37, gate=False))
+    check_attn(ctx, attn_case(12, [50, 9], 8, 2, 64, 16, "f16", prefix=20, scale=1e-45, gate=False))
 
 
 def test_attn_rows_that_see_nothing(ctx):
