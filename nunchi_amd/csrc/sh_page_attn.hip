@@ -2,6 +2,11 @@
 // one matrix product for all query rows, and each request's own. Parts of the keys are taken by workgroups of their own
 // (k_page_attn) and joined after them (k_page_join): with a part's maximum m, sum l of e^(s - m) and sum O of e^(s - m) v,
 // two parts have m' = max(m1, m2), l' = l1 e^(m1 - m') + l2 e^(m2 - m'), O' likewise, and the result is O / l.
+//
+// What bounds it: one row a request, memory (256 requests of up to 2048 own positions, 8 kv heads of 64: 607 MB in 120 us,
+// 5.05 TB/s, as a copy; the shared 8192 positions for all 8192 columns alone take 40 us, together with the own ones 159, and the
+// join 7); many rows, the exponentials and masks between the two products (VALU instructions outlast the matrix ones
+// two to one at head_dim 64); a few short requests, the launch (two behind 90 positions: 6.5 us of kernel).
 #include <hip/hip_runtime.h>
 
 #include <climits>
@@ -386,11 +391,12 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, joi
     }
 }
 
-// waves per SIMD that the registers are to allow
+// waves per SIMD that the registers are to allow: two where a workgroup holds 32 columns of 128 or 64 of 64 (256 requests behind
+// 8192 positions 166 us; 32 columns of 64 at three or four waves 185 to 190, as each key feeds half the products)
 constexpr int waves_of(int D, int nts, int nto) { return nts > 1 || nto > 1 ? 2 : D > 64 ? 3 : 4; }
 
 // Shared and own parts in one launch, eight workgroups of either in turn (one for each XCD): the shared ones wait for the
-// matrix units, the own ones for memory, and together they take little longer than the longer of the two alone.
+// matrix units and the VALU, the own ones for memory (166 us for both at 256 requests; 173 as two launches).
 template <class T, int D, int NTS, int NTO>
 __global__ __launch_bounds__(256, waves_of(D, NTS, NTO)) void k_page_attn(pattn_args a) {
     __shared__ __align__(16) union { join_space<D, NTO> own; join_space<D, NTS ? NTS : 1> shared; } js;
@@ -410,7 +416,9 @@ __global__ __launch_bounds__(256, waves_of(D, NTS, NTO)) void k_page_attn(pattn_
 }
 
 // One wave per (row, query head), or all four for many parts: lanes take four dimensions each, as many parts at once as
-// fit a wave
+// fit a wave. All four from 17 parts on: a wave alone reads them in turns that wait for each other (one request of 65521
+// positions, 32 heads: 7.5 us, a wave alone 20). With few parts the other waves only cost (256 requests of 32 heads: 7.3 us, four
+// waves 14; 48 of 16: 5.6 and 5.0).
 template <class T, int D, bool MANY>
 __global__ __launch_bounds__(256) void k_page_join(pattn_args a) {
     constexpr int LP = D / 4, AT_ONCE = 64 / LP, WAVES = MANY ? 4 : 1;   // lanes per part, parts at once
@@ -465,7 +473,8 @@ __global__ __launch_bounds__(256) void k_page_join(pattn_args a) {
     if (a.lse && d == 0) a.lse[rh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
-// column groups of 16 a workgroup takes: one, or as many as the registers hold
+// column groups of 16 a workgroup takes: one, or as many as the registers hold (prompts of 300 rows, head_dim 128: 40 us
+// in tiles of 32 columns, 84 in tiles of 16, which read every key twice as often)
 constexpr int many(int D) { return D > 64 ? 2 : 4; }
 int col_groups(int D, long long cols) { return cols <= 16 ? 1 : many(D); }
 
@@ -509,13 +518,15 @@ void split(long long base, long long range, long long want, int* parts, int* chu
 }  // namespace
 
 // Which workgroups take the shared positions, and into how many parts the keys go: about four workgroups per compute
-// unit, of 256 keys or more.
+// unit (two for the shared positions), of 256 keys or more. With twice as many parts 48 requests of 4096 positions took 63 to
+// 66 us instead of 62, the prompts below 76 instead of 40.
 bool page_attn_split(int D, bool single, pattn_args& a) {
     const int nto = col_groups(D, (long long)a.max_rows * a.grp);
     const long long own = own_tiles(a, nto, single), all = shared_tiles(a, col_groups(D, (long long)a.rows * a.grp));
     a.own_at = (a.prefix_len + 31) / 32 * 32;
     // Requests whose columns fill their workgroups read the shared positions themselves: sharing would not save reads,
-    // and nothing has to be joined. So do few requests with few shared positions
+    // and nothing has to be joined (13 prompts of 300 rows behind 500 positions: 40 us, 138 apart). So do few requests with
+    // few shared positions (two behind 90: 9.6 us a call, 20.8 with parts and a join)
     a.fused = a.prefix_len == 0 || own <= all * 2 || own * a.prefix_len <= 4096;
     a.sp = a.pchunk = 0;
     long long blocks = (long long)a.rows * a.n_head;
