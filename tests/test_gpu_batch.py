@@ -106,7 +106,7 @@ def plan_case(seed, n, page, most_held, most_add, spare=0):
 
 
 @pytest.mark.parametrize("n,page,held,add", [(1, 16, 0, 1), (1, 16, 40, 0), (2, 16, 15, 1), (3, 32, 31, 33), (64, 64, 300, 1), (255, 16, 100, 5),
-                                             (256, 16, 100, 70), (257, 128, 1000, 300), (1000, 256, 700, 3), (4096, 16, 60, 9)])
+                                             (256, 16, 100, 70), (3, 16, 40, 5), (5, 16, 100, 27), (2, 16, 3, 9000), (257, 128, 1000, 300), (1000, 256, 700, 3), (4096, 16, 60, 9)])
 def test_plan(ctx, n, page, held, add):
     h, a, table, free = plan_case(n * page, n, page, held, add)
     check_plan(ctx, h, a, page, table, free, 2, int(a.sum()), pos0=11)
