@@ -773,6 +773,12 @@ def test_engine_on_the_default_stream(tiny_model):
             (ha, la, ia), (hb, lb, ib) = a.step(tok), b.step(tok)
             assert np.array_equal(ha, hb) and np.array_equal(la, lb) and ia == ib
         assert np.array_equal(a.generate(5, 6)[0], b.generate(5, 6)[0])
+        u = np.random.default_rng(2).uniform(size=7)
+        assert np.array_equal(a.generate_sampled(8, u, top_k=30)[0], b.generate_sampled(8, u, top_k=30)[0])
+        # (a longer call after a shorter one, and a shorter one again)
+        u = np.random.default_rng(3).uniform(size=20)
+        x, y = (z.generate_sampled(9, u, a=z.new_state())[0] for z in (a, b))
+        assert np.array_equal(x, y) and np.array_equal(x[:5], b.generate_sampled(9, u[:5], a=b.new_state())[0])
 
 
 @pytest.mark.parametrize("kw", [dict(), dict(temp=0.7, top_k=20), dict(top_p=0.8, temp=1.3), dict(min_p=0.1), dict(temp=0.0)], ids=str)
