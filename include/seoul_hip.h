@@ -404,7 +404,8 @@ int sh_page_attn(sh_ctx* ctx, const sh_page_shape* shape, int n, int rows, const
  * top_p, min_p is one value per row or null (1, 0, 1, 0). Scores of -inf or NaN are never taken; a score of +inf leaves
  * only those. A row with nothing to take, or whose temp is negative or NaN, gives -1 and chance 0. A NaN in u, top_p or
  * min_p counts as 0, 1, 0. Weights are summed in 2^-44ths of the largest (smaller ones are never taken), vocab is at most
- * 524288. sh_generate picks greedily, sh_voice_sample samples codes. work: sh_sample_work's bytes, as above. */
+ * 524288. sh_generate picks greedily, sh_voice_sample samples codes. work: sh_sample_work's bytes, as above (256:
+ * a workgroup keeps its row to itself; it is there for rows shared among several). */
 int sh_sample_work(int rows, int vocab, size_t* bytes);
 int sh_sample(sh_ctx* ctx, int rows, int vocab, const void* scores, long long ld, int type, const float* temp,
               const int32_t* top_k, const float* top_p, const float* min_p, const double* u, int32_t* ids, float* chance,
