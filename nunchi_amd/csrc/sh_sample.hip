@@ -49,6 +49,9 @@ __device__ __forceinline__ u64 fixed(float w) {
     const float h = w * 4096.0f;
     return ((u64)(unsigned)h << 32) | (unsigned)(__builtin_amdgcn_fractf(h) * 4294967296.0f);
 }
+// the least weight that counts: below it a word has none in 2^-44ths, and is never taken
+constexpr float LEAST_WEIGHT = 0x1p-44f;
+__device__ __forceinline__ float counted(float w) { return w >= LEAST_WEIGHT ? w : 0.0f; }
 // of n equal words of weight w each, those before which the sum is still below `left`: one at least
 __device__ __forceinline__ u64 words_left(double left, u64 w, u64 n) {
     const u64 r = w && left > 0.0 ? (u64)ceil(left / (double)w) : 1;
@@ -660,7 +663,7 @@ __global__ __launch_bounds__(ST) void k_sample(sample_args a) {
                         each([&](const float* v, int, int k) {
                             float part = 0.0f;
 #pragma unroll
-                            for (int e = 0; e < V; e++) part += v[e] >= low ? weight(v[e]) : 0.0f;
+                            for (int e = 0; e < V; e++) part += v[e] >= low ? counted(weight(v[e])) : 0.0f;
                             put(part, k);
                         });
                     } else {
@@ -672,7 +675,7 @@ __global__ __launch_bounds__(ST) void k_sample(sample_args a) {
                             for (int e = 0; e < V; e++) {
                                 const float d = top - v[e], f = fmaf(d, ch, d * cl);
                                 const bool above = f < f0;
-                                part += above ? __builtin_amdgcn_exp2f(-f) : 0.0f;
+                                part += above ? counted(__builtin_amdgcn_exp2f(-f)) : 0.0f;
                                 bits |= f < f1 && !above ? 1u << e : 0u;
                             }
                             mark(k, bits);
@@ -772,7 +775,7 @@ __global__ __launch_bounds__(ST) void k_sample(sample_args a) {
                 }
                 __syncthreads();
                 id = w.template pick<V>(s.blocks, nb, [&](int at, float* v) { words.load(at, v); },
-                                        [&](float x, int i) { return kept(x, i) ? (double)weight(x) * 17592186044416.0 : 0.0; },
+                                        [&](float x, int i) { return kept(x, i) ? (double)mass(x) : 0.0; },
                                         [&](u64 total) { return target(q.u, total); }, sum);
                 won = weight_of(((double)top - (double)(float)words.x[id]) * c);
             }

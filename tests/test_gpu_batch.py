@@ -968,3 +968,30 @@ def test_tensors_are_checked(ctx):
         nunchi_amd.page_attn(ctx, c["shape"], c["q"], c["keys"], c["values"], c["table"], c["length"], c["out"], work, 20, prefix=c["shared"][:1], prefix_len=20)
     with pytest.raises(ValueError):
         run_attn(ctx, {**c, "keys": c["keys"][1:]})
+
+
+LOW_LAYOUTS = [(700, "f32"), (40000, "f32"), (120000, "f32"), (1000, "bf16"), (70001, "f16"), (262144, "bf16")]
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=20), dict(top_k=300), dict(top_p=0.9), dict(top_k=12, top_p=0.8), dict(min_p=0.01), dict(temp=1.3)], ids=str)
+@pytest.mark.parametrize("vocab,kind", LOW_LAYOUTS)
+def test_sample_never_takes_words_without_weight(ctx, vocab, kind, kw):
+    """Words 300 and more below the maximum (2^-432 of it: no weight in 2^-44ths) first and last in every block, u at the ends of
+    its range: none of them is taken, whatever holds the row."""
+    g = torch.Generator().manual_seed(vocab)
+    u = [0.0, -1.0, math.nan, 1.0, 2.0, np.nextafter(1.0, 0.0), 1e-300, 0.5, 0.77]
+    x = torch.full((len(u), vocab), -math.inf)
+    for at in (0, 1, 255, 256, 511, 512):
+        x[:, at::1024] = -300.0 - at
+    x[:, 255::256], x[:, ::256], x[:, -1] = -1000.0, -60000.0, -60000.0
+    good = torch.randperm(vocab, generator=g)[:60]
+    x[:, good] = 5 + torch.randn(len(u), 60, generator=g)
+    x = x.to(TYPES[kind])
+    ids, chance = run_sample(ctx, x.cuda(), u, **kw)
+    x = x.double().numpy()
+    x[x < -100] = -np.inf
+    kw = {k: v if k == "top_k" else np.float32(v).item() for k, v in kw.items()}
+    for r in range(len(u)):
+        want, c = sample_reference(x[r], u[r], **kw)
+        assert ids[r] == want, (r, ids[r], want)
+        assert chance[r] > 0 and abs(chance[r] - c) <= 2.0 ** -21 * c, (r, chance[r], c)
