@@ -7,16 +7,18 @@
 // weights' exponent (-log2 w in 64ths of a power of two, 4096 bins in LDS) tells the bin that holds the cut; its words,
 // a few dozen, are listed and each counts those before it. The pick is a search for the running sum in index order,
 // first over the sums of blocks of 64 lanes' words, then within one.
-// Histogram weights are summed as integers, in 2^-44ths of the largest: their sums do not depend on the order of the
-// atomics. Block sums are formed in a fixed order. So a row's word is the same every time.
+// Weights are summed as integers, in 2^-44ths of the largest, in histograms and blocks alike: sums do not depend on the
+// order of the atomics, a block's is exactly its words', and a row's word is the same every time. (Blocks summed in single
+// precision, as before, lost words of 2^-24 of a block; the integers cost 3 to 4 us of the figures below.)
 //
-// A workgroup holds a row in registers: it is read from memory once (256 rows of 97496 fp32 scores: 20 us
-// at 5 TB/s), and every pass over it after that costs instructions, which bound it: 256 such rows take 22 us at temperature
-// 0, 31 with no filter or top-k 50, 53 to 62 with top-p 0.9, 58 mixed; one row 19. Up to 32768 32-bit words 1024 threads hold 32 each (61 rows of 32003 bf16 scores 18 us; 71 where
-// each pass read them again). Up to 98304 words 512 threads hold 192 each, as many as the registers leave: 1024 threads would have
-// 128 registers a thread and spill. Above, and for the rare rows that need it (+inf among the scores, more than 4096 words
-// listed by top-k or 512 in the cut's bin, scores further apart than 2^64 in weight at the cut), every step reads the row
-// again, which the caches hold by then (sample_again; top-k 5000 of 97496: 255 us for 256 rows).
+// A workgroup holds a row in registers: it is read from memory once (256 rows of 97496 fp32 scores: 20 us at 5 TB/s), and
+// every pass over it after that costs instructions, which bound it: 256 such rows take 22 us at temperature 0, 31 with
+// top-k 50, 35 with no filter, 55 to 65 with top-p 0.9, 62 mixed; one row 21. Up to 32768 32-bit words 1024 threads hold 32
+// each (61 rows of 32003 bf16 scores 19 us with top-p; 71 where each pass read them again). Up to 98304 words 512 threads
+// hold 192 each, as many as the registers leave: 1024 threads would have 128 registers a thread and spill. Above, and for
+// the rare rows that need it (+inf among the scores, more than 4096 words listed by top-k or 512 in the cut's bin, scores
+// further apart than 2^64 in weight at the cut), every step reads the row again, which the caches hold by then
+// (sample_again; top-k 5000 of 97496: 265 us for 256 rows).
 #include <hip/hip_runtime.h>
 
 #include "sh_device.h"
@@ -49,9 +51,16 @@ __device__ __forceinline__ u64 fixed(float w) {
     const float h = w * 4096.0f;
     return ((u64)(unsigned)h << 32) | (unsigned)(__builtin_amdgcn_fractf(h) * 4294967296.0f);
 }
-// the least weight that counts: below it a word has none in 2^-44ths, and is never taken
-constexpr float LEAST_WEIGHT = 0x1p-44f;
-__device__ __forceinline__ float counted(float w) { return w >= LEAST_WEIGHT ? w : 0.0f; }
+// the same as two numbers of 22 bits whose sums over a block (512 words at most) fit 32: a word's cost no carries
+struct halves {
+    unsigned hi = 0, lo = 0;
+    __device__ __forceinline__ void add(float w) {
+        const float h = w * 4194304.0f;
+        hi += (unsigned)h;
+        lo += (unsigned)(__builtin_amdgcn_fractf(h) * 4194304.0f);
+    }
+    __device__ __forceinline__ u64 sum() const { return ((u64)hi << 22) + lo; }
+};
 // of n equal words of weight w each, those before which the sum is still below `left`: one at least
 __device__ __forceinline__ u64 words_left(double left, u64 w, u64 n) {
     const u64 r = w && left > 0.0 ? (u64)ceil(left / (double)w) : 1;
@@ -273,26 +282,18 @@ template <int ST> struct row_search {
         }
         __syncthreads();
         if (t < 64) {
-            typedef decltype(of(0.0f, 0)) num;
             float v[V];
-            num w[V], own = 0;
+            u64 w[V], own = 0;
             const int w0 = ((int)found[1] * 64 + lane) * V;
             load(w0, v);
 #pragma unroll
             for (int e = 0; e < V; e++) own += w[e] = of(v[e], w0 + e);
-            const num in = wave_scan(own);
-            num before = (num)found[2] + in - own;
-            // (a block's sum may be rounded otherwise than its words' are: past its end the last kept word is taken)
-            const unsigned long long some = __ballot(own != 0), past = __ballot(own != 0 && (num)target < before + own);
-            const int who = past ? __ffsll(past) - 1 : 63 - __clzll(some);
-            if (lane == who) {
-                int last = 0, e = 0;
-                for (; e < V; e++) {
-                    if (w[e]) last = e;
-                    before += w[e];
-                    if (w[e] && (num)target < before) break;
-                }
-                found[3] = (u64)(w0 + last);
+            u64 before = found[2] + wave_scan(own) - own;
+            // (the block's sum is its words': one lane holds the target, at a word of some weight)
+            if (before <= target && target < before + own) {
+                int e = 0;
+                while (before + w[e] <= target) before += w[e++];
+                found[3] = (u64)(w0 + e);
             }
         }
         __syncthreads();
@@ -653,36 +654,37 @@ __global__ __launch_bounds__(ST) void k_sample(sample_args a) {
                     for (int b = t; b < nb; b += ST) s.blocks[b] = 0;
                 } else {
                     // the weights above the cut's bin summed up by blocks, the words of the bin listed
-                    float sums = 0.0f;     // lane k: the sum of the wave's words of slab k
-                    auto put = [&](float part, int k) {
-                        part = wave_scan(part);
-                        const float whole = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(part), 63));
-                        sums = lane == k ? whole : sums;
+                    halves sums;           // lane k: the sum of the wave's words of slab k
+                    auto put = [&](halves part, int k) {
+                        const unsigned hi = (unsigned)__builtin_amdgcn_readlane((int)wave_scan(part.hi), 63);
+                        const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)wave_scan(part.lo), 63);
+                        sums.hi = lane == k ? hi : sums.hi;
+                        sums.lo = lane == k ? lo : sums.lo;
                     };
                     if (b0 < 0) {
                         each([&](const float* v, int, int k) {
-                            float part = 0.0f;
+                            halves part;
 #pragma unroll
-                            for (int e = 0; e < V; e++) part += v[e] >= low ? counted(weight(v[e])) : 0.0f;
+                            for (int e = 0; e < V; e++) part.add(v[e] >= low ? weight(v[e]) : 0.0f);
                             put(part, k);
                         });
                     } else {
                         const float f0 = (float)b0 * (64.0f / BINS), f1 = (float)(b0 + 1) * (64.0f / BINS);   // (exact)
                         each([&](const float* v, int, int k) {
-                            float part = 0.0f;
+                            halves part;
                             unsigned bits = 0;
 #pragma unroll
                             for (int e = 0; e < V; e++) {
                                 const float d = top - v[e], f = fmaf(d, ch, d * cl);
                                 const bool above = f < f0;
-                                part += above ? counted(__builtin_amdgcn_exp2f(-f)) : 0.0f;
+                                part.add(above ? __builtin_amdgcn_exp2f(-f) : 0.0f);
                                 bits |= f < f1 && !above ? 1u << e : 0u;
                             }
                             mark(k, bits);
                             put(part, k);
                         });
                     }
-                    if (lane * SW + wv < nb) s.blocks[lane * SW + wv] = (u64)((double)sums * 17592186044416.0);
+                    if (lane * SW + wv < nb) s.blocks[lane * SW + wv] = sums.sum();
                     if (b0 >= 0) {
                         list_marked(&s.n_near, NEAR, [&](unsigned k, int i) { s.near[k].i = i; });
                         if (!again)
@@ -775,7 +777,7 @@ __global__ __launch_bounds__(ST) void k_sample(sample_args a) {
                 }
                 __syncthreads();
                 id = w.template pick<V>(s.blocks, nb, [&](int at, float* v) { words.load(at, v); },
-                                        [&](float x, int i) { return kept(x, i) ? (double)mass(x) : 0.0; },
+                                        [&](float x, int i) -> u64 { return kept(x, i) ? mass(x) : 0; },
                                         [&](u64 total) { return target(q.u, total); }, sum);
                 won = weight_of(((double)top - (double)(float)words.x[id]) * c);
             }

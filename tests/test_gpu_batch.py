@@ -995,3 +995,30 @@ def test_sample_never_takes_words_without_weight(ctx, vocab, kind, kw):
         want, c = sample_reference(x[r], u[r], **kw)
         assert ids[r] == want, (r, ids[r], want)
         assert chance[r] > 0 and abs(chance[r] - c) <= 2.0 ** -21 * c, (r, chance[r], c)
+
+
+@pytest.mark.parametrize("vocab,kind", LOW_LAYOUTS)
+def test_sample_small_weights_beside_a_large_one(ctx, vocab, kind):
+    """255 words of e^-18 (one of e^-20) in the block of one of weight 1, and u inside the k-th one's share: sums in 2^-44ths tell
+    them apart. A small weight is 2^-26 (2^-28.9), its last place 2^-18 (2^-15) of it and its exponential's 2^-22, so 255 of them
+    are off by less than 1/500 of one; u is 1/4 of one from the next."""
+    g = torch.Generator().manual_seed(1)
+    k = torch.randint(0, 255, (24,), generator=g).numpy()
+    e = math.exp(-18.0)
+    x = torch.full((24, vocab), -math.inf)
+    x[:, :256] = -18.0
+    x[:, 128] = 0.0
+    total = 1 + 255 * e
+    u = np.where(k < 128, (k + 0.25) * e, 1 + (k + 0.25) * e) / total
+    want = k + (k >= 128)
+    x = x.to(TYPES[kind]).cuda()
+    for kw in (dict(), dict(min_p=1e-9), dict(top_k=256)):
+        ids, _ = run_sample(ctx, x, u, **kw)
+        assert np.array_equal(ids, want), kw
+    # one small word, last of the block and of the row
+    for at in (255, vocab - 1):
+        x = torch.full((6, vocab), -math.inf)
+        x[:, 0], x[:, at] = 0.0, -20.0
+        ids, chance = run_sample(ctx, x.to(TYPES[kind]).cuda(), [1.0, 1 - 1e-9, np.nextafter(1.0, 0.0), 1 - 3e-9, 0.0, 3.0])
+        assert ids.tolist() == [at, at, at, 0, 0, at]
+        assert abs(chance[0] / math.exp(-20.0) - 1) < 2.0 ** -21
