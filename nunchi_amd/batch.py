@@ -38,7 +38,11 @@ class PageShape(C.Structure):
         if dtype not in _TYPES:
             raise ValueError("pages hold f16 or bf16")
         super().__init__(int(n_head), int(n_kv), int(head_dim), int(page), _TYPES[dtype], int(window), int(n_pages), float(scale), float(eps))
-        self.address = C.addressof(self)
+
+    @property
+    def address(self) -> int:
+        """Where this object's fields are (a copy's are its own: the address is not kept)."""
+        return C.addressof(self)
 
     @property
     def cache_shape(self) -> tuple:

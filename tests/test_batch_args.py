@@ -1,6 +1,10 @@
 """Refusals of the batch operators (sh_page_plan, sh_page_put, sh_page_attn, sh_sample) that need no GPU: every check below
 comes before the context or any buffer is touched, so the context and the buffers here are addresses only."""
+import copy
 import ctypes as C
+import gc
+import pickle
+from types import SimpleNamespace
 
 import pytest
 
@@ -142,3 +146,25 @@ def test_create_on_refuses_like_create():
     assert _lib().sh_create_on(-1, None, C.byref(h)) != 0
     with pytest.raises(nunchi_amd.SeoulError):
         nunchi_amd.Context(4096, stream=0)
+
+
+@pytest.mark.parametrize("way", [copy.copy, copy.deepcopy, lambda s: pickle.loads(pickle.dumps(s))], ids=["copy", "deepcopy", "pickle"])
+def test_a_copied_shape_is_the_one_a_call_reads(way):
+    """What a call reads is the copy's own: its page count (11, the original's is 10) and window, also once the original is gone.
+    The tensors are host memory and have no rows, so the call ends before it touches the context."""
+    torch = pytest.importorskip("torch")
+    first = shape()
+    second = way(first)
+    second.n_pages, second.window = 11, 256
+    assert second.address == C.addressof(second) and first.address == C.addressof(first) != second.address
+    assert PageShape.from_address(second.address).window == 256 and PageShape.from_address(first.address).window == 0
+    del first
+    gc.collect()
+    ctx = SimpleNamespace(h=SimpleNamespace(value=BASE), device=-1)
+    keys, values = (torch.zeros(second.cache_shape, dtype=torch.float16) for _ in range(2))
+    nunchi_amd.page_put(ctx, second, torch.zeros(0, 768), torch.zeros(0, dtype=torch.int64), keys, values)
+    with pytest.raises(ValueError, match="11"):
+        nunchi_amd.page_put(ctx, second, torch.zeros(0, 768), torch.zeros(0, dtype=torch.int64), keys[1:], values[1:])
+    out = torch.zeros(0, 8, 64, dtype=torch.float16)
+    nunchi_amd.page_attn(ctx, second, out, keys, values, torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), out.clone(),
+                         torch.zeros(256, dtype=torch.uint8), 4, cu=torch.zeros(3, dtype=torch.int32))
