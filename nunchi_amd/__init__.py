@@ -416,6 +416,8 @@ class Brain:
         u = np.ascontiguousarray(u, np.float64)
         n = u.size
         if b is not None:
+            if u_b is None:
+                raise ValueError("u_b is missing: b's words need random numbers of their own")
             u_b = np.ascontiguousarray(u_b, np.float64)
             if u_b.size != n:
                 raise ValueError("u and u_b must hold as many random numbers")

@@ -168,3 +168,12 @@ def test_a_copied_shape_is_the_one_a_call_reads(way):
     out = torch.zeros(0, 8, 64, dtype=torch.float16)
     nunchi_amd.page_attn(ctx, second, out, keys, values, torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), out.clone(),
                          torch.zeros(256, dtype=torch.uint8), 4, cu=torch.zeros(3, dtype=torch.int32))
+
+
+def test_generate_sampled_wants_the_second_conversations_random_numbers():
+    """Refused before anything is called, also for one step (where a missing array would pass for one number, NaN)."""
+    brain = nunchi_amd.Brain.__new__(nunchi_amd.Brain)      # (a model needs a GPU)
+    brain.state, other = SimpleNamespace(), SimpleNamespace()
+    for u in ([0.5], [0.5, 0.25], []):
+        with pytest.raises(ValueError, match="u_b"):
+            brain.generate_sampled(3, u, b=other, first_b=4)
