@@ -529,7 +529,6 @@ bool page_attn_split(int D, bool single, pattn_args& a) {
     // few shared positions (two behind 90: 9.6 us a call, 20.8 with parts and a join)
     a.fused = a.prefix_len == 0 || own <= all * 2 || own * a.prefix_len <= 4096;
     a.sp = a.pchunk = 0;
-    long long blocks = (long long)a.rows * a.n_head;
     if (!a.fused) {
         const long long range = a.window && a.window + 31ll < a.prefix_len ? a.window + 31ll : a.prefix_len;
         split(all * a.n_kv, range, 512, &a.sp, &a.pchunk);
@@ -541,9 +540,9 @@ bool page_attn_split(int D, bool single, pattn_args& a) {
     }
     split(own * a.n_kv, range, 1024, &a.so, &a.ochunk);
     const long long shared_blocks = all * a.n_kv * a.sp, own_blocks = own * a.n_kv * a.so;
-    if (shared_blocks + own_blocks + 16 > blocks) blocks = shared_blocks + own_blocks + 16;
+    const long long rh = (long long)a.rows * a.n_head, join = a.sp + a.so == 1 ? 0 : a.sp + a.so > 16 ? rh : (rh + 3) / 4;
     // (columns of one kv head are counted in 32 bits in the kernel)
-    if (blocks > INT_MAX || (long long)a.rows * a.grp > INT_MAX / 2) return false;
+    if (shared_blocks + own_blocks + 16 > most_blocks(256) || join > most_blocks(256) || (long long)a.rows * a.grp > INT_MAX / 2) return false;
     a.shared_blocks = (int)shared_blocks;
     a.own_blocks = (int)own_blocks;
     return true;

@@ -12,6 +12,9 @@ enum { TY_F32 = 0, TY_F16 = 1, TY_BF16 = 30 };
 constexpr int PLAN_MAX_N = 4096;   // requests of a step: their running sums live in LDS
 constexpr int SAMPLE_MAX_VOCAB = 1 << 19;   // 2^44 times as many fits 64 bits
 
+// the workgroups of so many threads that one launch holds (less than 2^32 threads)
+constexpr long long most_blocks(int threads) { return 0xFFFFFFFFll / threads; }
+
 struct plan_args {
     int n, page_log, cols, n_free, rows, pos0;
     const int32_t *held, *add, *free_pages, *taken;

@@ -165,7 +165,7 @@ int sh_page_put(sh_ctx* c, const sh_page_shape* s, int rows, const void* qkv, lo
     const long long heads = (long long)s->n_head + 2ll * s->n_kv;
     if (ld < heads * s->head_dim) return bad(who, "a row (ld) is shorter than its heads");
     if (rope && n_rope < 1) return bad(who, "n_rope must be positive");
-    if ((rows * heads + 15) / 16 > INT_MAX) return bad(who, "more rows than one launch holds");
+    if ((rows * heads + 15) / 16 > most_blocks(256)) return bad(who, "more rows than one launch holds");
     if (off(qkv, src_type == SH_F32 ? 4 : 2)) return bad(who, "qkv is not aligned to its type");
     if (off(q_out, 16) || off(keys, 16) || off(values, 16)) return bad(who, "queries, keys and values start on 16 bytes");
     const size_t cache = (size_t)s->n_pages * s->n_kv * s->page * s->head_dim * 2, vec = (size_t)s->head_dim * 4;
@@ -201,15 +201,22 @@ int sh_page_attn_work(const sh_page_shape* s, int n, int rows, int max_rows, int
     SH_ENTRY
     if (!bytes) return bad("sh_page_attn_work", "null");
     *bytes = 0;
-    // (with or without cu: what either needs)
+    // (with or without cu: what either needs, of those that one launch holds)
+    const char* fault = nullptr;
+    bool any = false;
     for (const bool single : {false, true}) {
         if (single && (rows != n || max_rows != 1)) continue;
         pattn_args a{};
-        if (const char* f = attn_sizes(s, n, rows, max_rows, prefix_len, max_len, single, a)) return bad("sh_page_attn_work", f);
+        if (const char* f = attn_sizes(s, n, rows, max_rows, prefix_len, max_len, single, a)) {
+            fault = f;
+            continue;
+        }
+        any = true;
         size_t sums, all;
         attn_work(a, s->head_dim, &sums, &all);
         if (all > *bytes) *bytes = all;
     }
+    if (!any) return bad("sh_page_attn_work", fault);
     if (*bytes < 256) *bytes = 256;
     return SH_OK;
     SH_ENTRY_END
@@ -259,6 +266,7 @@ int sh_sample_work(int rows, int vocab, size_t* bytes) {
     if (!bytes) return bad("sh_sample_work", "null");
     *bytes = 0;
     if (rows < 0 || vocab < 1 || vocab > SAMPLE_MAX_VOCAB) return bad("sh_sample_work", "rows is negative, or vocab not 1 to 524288");
+    if (rows > most_blocks(1024)) return bad("sh_sample_work", "more rows than one launch holds");
     *bytes = 256;
     return SH_OK;
     SH_ENTRY_END

@@ -177,3 +177,23 @@ def test_generate_sampled_wants_the_second_conversations_random_numbers():
     for u in ([0.5], [0.5, 0.25], []):
         with pytest.raises(ValueError, match="u_b"):
             brain.generate_sampled(3, u, b=other, first_b=4)
+
+
+def test_launches_of_2_to_the_32_threads_are_refused():
+    """A launch holds less than 2^32 threads: 2^24 - 1 workgroups of 256 for attention and writes, 2^22 - 1 rows of 1024 for
+    sampling. What passes that is an argument error of the size functions and the calls, before anything runs."""
+    L, size = _lib(), C.c_size_t()
+    s = shape(n_head=65536, n_kv=65536, n_pages=1000)      # (a workgroup for each row and head)
+    assert L.sh_page_attn_work(C.byref(s), 255, 255, 1, 0, 100, C.byref(size)) == 0
+    assert L.sh_page_attn_work(C.byref(s), 256, 256, 1, 0, 100, C.byref(size)) == ARG
+    assert b"fewer rows" in L.sh_last_error()
+    s = shape(n_head=16, n_kv=16)
+    assert L.sh_page_attn_work(C.byref(s), 1 << 22, 1 << 22, 1, 4096, 100, C.byref(size)) == ARG
+    assert b"fewer rows" in L.sh_last_error()
+    s = shape(n_head=14, n_kv=1)                           # (a workgroup for each row of 16 heads)
+    assert L.sh_page_put(BASE, C.byref(s), 1 << 24, at(0), 1024, 0, None, None, None, 0, None, at(1), None, at(2), at(3)) == ARG
+    assert b"more rows" in L.sh_last_error()
+    assert L.sh_sample_work((1 << 22) - 1, 10, C.byref(size)) == 0
+    assert L.sh_sample_work(1 << 22, 10, C.byref(size)) == ARG
+    assert L.sh_sample(BASE, 1 << 22, 10, at(0), 10, 0, None, None, None, None, at(1), at(2), None, at(3), 256) == ARG
+    assert b"rows" in L.sh_last_error()
