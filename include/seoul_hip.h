@@ -137,9 +137,10 @@ int sh_file_block(const sh_file* f, const void** data, size_t* size);
 /* ---- engine: imi_seoul::load / reset / step / step2 / step_batch / new_state / swap_state ---- */
 int sh_create(int device, sh_ctx** out);
 /* The same on the caller's own stream (a hipStream_t of `device`; null: the device's default stream): everything the
- * context enqueues runs in order with the caller's other work there, and a graph captured on that stream holds it. The
- * stream must outlive the context, which does not destroy it. On the default stream, which cannot be captured, the
- * engine's steps run without their graph (the same kernels, the same numbers). */
+ * context enqueues runs in order with the caller's other work there. A graph that the caller captures on that stream holds
+ * the calls that do not wait (the batch operators, sh_q4_gemv_dev and the like); calls that wait for their results, the
+ * engine's steps among them, cannot be captured. The engine makes its own graphs on a stream of its own, so other threads
+ * may enqueue on the caller's meanwhile. The stream must outlive the context, which does not destroy it. */
 int sh_create_on(int device, void* stream, sh_ctx** out);
 int sh_destroy(sh_ctx* ctx);
 /* Read a GGUF brain file, repack every Q4_0 table into the device layout and upload it; n_ctx = context length of

@@ -299,6 +299,24 @@ int enqueue_step(sh_ctx* c, int M, bool want_logits) {
     return SH_OK;
 }
 
+// A capture takes in whatever is enqueued on its stream meanwhile, and the stream may be the caller's, on which another
+// thread works: what is captured goes through a stream of its own, the context's while this lives
+struct capture_stream {
+    sh_ctx* c;
+    hipStream_t usual, own = nullptr;
+    hipError_t e;
+    explicit capture_stream(sh_ctx* ctx) : c(ctx), usual(ctx->stream) {
+        e = hipStreamCreateWithFlags(&own, hipStreamNonBlocking);
+        if (e == hipSuccess) c->stream = own;
+    }
+    ~capture_stream() {
+        c->stream = usual;
+        if (own) (void)hipStreamDestroy(own);
+    }
+    capture_stream(const capture_stream&) = delete;
+    capture_stream& operator=(const capture_stream&) = delete;
+};
+
 int get_graph(sh_ctx* c, int M, bool want_logits, hipGraphExec_t* out) {
     if (!c->use_graphs) {
         *out = nullptr;
@@ -307,6 +325,8 @@ int get_graph(sh_ctx* c, int M, bool want_logits, hipGraphExec_t* out) {
     hipGraphExec_t& g = c->graph[M][want_logits ? 1 : 0];
     if (!g) {
         hipGraph_t graph = nullptr;
+        const capture_stream own(c);
+        HIPCHK(own.e);
         HIPCHK(hipStreamBeginCapture(c->stream, hipStreamCaptureModeThreadLocal));
         const int rc = enqueue_step(c, M, want_logits);
         hipError_t e = hipStreamEndCapture(c->stream, &graph);
@@ -477,7 +497,7 @@ static int create(int device, bool own_stream, hipStream_t stream, sh_ctx** out)
     HIPCHK(hipMalloc((void**)&c->P_dev, sizeof(step_params)));
     memset(c->P_host, 0, sizeof(step_params));
     const char* g = getenv("SEOUL_HIP_GRAPHS");
-    c->use_graphs = !(g && g[0] == '0') && (own_stream || stream);   // (the default stream cannot be captured)
+    c->use_graphs = !(g && g[0] == '0');
     const char* pf = getenv("SEOUL_HIP_PREFILL");
     c->use_prefill = !(pf && strcmp(pf, "0") == 0);
     const char* pc = getenv("SEOUL_HIP_PRECUT");
@@ -1591,10 +1611,15 @@ int sh_q4_bench_graph(sh_ctx* c, sh_q4* const* tables, int n_tables, int n_in, i
     // one pass over the tables, captured once: every launch a graph node behind the one before it
     hipGraph_t graph = nullptr;
     hipGraphExec_t exec = nullptr;
-    HIPCHK(hipStreamBeginCapture(c->stream, hipStreamCaptureModeThreadLocal));
     int rc = SH_OK;
-    for (int i = 0; i < n_tables && rc == SH_OK; i++) rc = q4_gemv_launch(c, tables[i], c->bench_x, n_in, c->bench_y, cut_mode, nullptr, nullptr);
-    hipError_t e = hipStreamEndCapture(c->stream, &graph);
+    hipError_t e;
+    {
+        const capture_stream own(c);
+        HIPCHK(own.e);
+        HIPCHK(hipStreamBeginCapture(c->stream, hipStreamCaptureModeThreadLocal));
+        for (int i = 0; i < n_tables && rc == SH_OK; i++) rc = q4_gemv_launch(c, tables[i], c->bench_x, n_in, c->bench_y, cut_mode, nullptr, nullptr);
+        e = hipStreamEndCapture(c->stream, &graph);
+    }
     if (rc != SH_OK || e != hipSuccess) {
         if (graph) (void)hipGraphDestroy(graph);
         return rc != SH_OK ? rc : fail(SH_E_HIP, std::string("sh_q4_bench_graph: capture: ") + hipGetErrorString(e));

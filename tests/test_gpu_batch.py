@@ -15,6 +15,7 @@ Tolerances count roundings. HALF is half a step of a 16-bit type relative to the
  sample: ids are equal; the chance is a weight (2^-23) over an exact sum of such weights (2^-23 at most), rounded once.
 """
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -1022,3 +1023,41 @@ def test_sample_small_weights_beside_a_large_one(ctx, vocab, kind):
         ids, chance = run_sample(ctx, x.to(TYPES[kind]).cuda(), [1.0, 1 - 1e-9, np.nextafter(1.0, 0.0), 1 - 3e-9, 0.0, 3.0])
         assert ids.tolist() == [at, at, at, 0, 0, at]
         assert abs(chance[0] / math.exp(-20.0) - 1) < 2.0 ** -21
+
+
+def test_first_step_beside_work_on_the_same_stream(tiny_model):
+    """A brain on the caller's stream makes its graph while another thread enqueues there: what that thread enqueues runs once,
+    when it is its turn, and no replay of the graph repeats it."""
+    side = torch.cuda.Stream()
+    x = torch.zeros(64, device="cuda")
+    torch.cuda.synchronize()
+    stop, started, count, errors = threading.Event(), threading.Event(), [0], []
+
+    def other():
+        try:
+            with torch.cuda.stream(side):
+                while not stop.is_set():
+                    x.add_(1)
+                    count[0] += 1
+                    started.set()
+        except Exception as e:   # noqa: BLE001  (shown by the test's own thread)
+            errors.append(e)
+            started.set()
+
+    brains = [nunchi_amd.Brain(tiny_model, n_ctx=64, ctx=nunchi_amd.Context(0, stream=side.cuda_stream)) for _ in range(6)]
+    thread = threading.Thread(target=other)
+    thread.start()
+    try:
+        assert started.wait(60)
+        ids = [[b.step(t)[2] for t in (3, 141, 59)] for b in brains]
+    finally:
+        stop.set()
+        thread.join()
+    side.synchronize()
+    assert not errors, errors
+    assert (x == count[0]).all(), (x[0].item(), count[0])
+    assert all(i == ids[0] for i in ids)
+    for b in brains:
+        b.step(7)
+    side.synchronize()
+    assert (x == count[0]).all(), "a replay repeats the other thread's work"
