@@ -21,7 +21,7 @@ def _load():
     try:
         from . import _batch
     except ImportError as e:
-        raise ImportError("nunchi_amd/_batch.so is not built: run `python -m nunchi_amd.build`") from e
+        raise ImportError("nunchi_amd._batch is not built for this Python: run `python -m nunchi_amd.build` (it needs a C++ compiler and Python.h)") from e
     lib = _n.load_library()
     _native = (_batch, *(C.cast(getattr(lib, f), C.c_void_p).value for f in ("sh_page_plan", "sh_page_put", "sh_page_attn", "sh_sample")))
     return _native

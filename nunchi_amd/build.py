@@ -18,7 +18,8 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libseoul_hip.so")
-MODULE = os.path.join(HERE, "_batch.so")     # the batch operators' CPython module (checks of tensors; links nothing)
+# the batch operators' CPython module (checks of tensors; links nothing), for the Python that builds it
+MODULE = os.path.join(HERE, "_batch" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 SOURCES = ["csrc/sh_kernels.hip", "csrc/sh_voice.hip", "csrc/sh_prefill.hip", "csrc/sh_noalloc.hip", "csrc/sh_codec.hip",
            "csrc/sh_ears.hip", "csrc/sh_calib.hip", "csrc/sh_pages.hip", "csrc/sh_page_attn.hip", "csrc/sh_sample.hip",
            "csrc/sh_engine.cpp", "csrc/sh_codec_host.cpp", "csrc/sh_ears_host.cpp", "csrc/sh_voice_host.cpp",
@@ -67,19 +68,32 @@ def build(verbose: bool = False) -> str:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("hipcc failed linking libseoul_hip.so")
         os.replace(tmp, LIB)
-        tmp = MODULE + f".tmp{os.getpid()}"
-        cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-I", sysconfig.get_paths()["include"], "-o", tmp,
-               os.path.join(HERE, "csrc", "py_batch.cpp")]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            sys.stderr.write(r.stdout + r.stderr)
-            raise RuntimeError("compiling _batch.so failed")
-        os.replace(tmp, MODULE)
     finally:
         shutil.rmtree(tmpdir, ignore_errors=True)
+    build_module(verbose)
     return LIB
+
+
+def build_module(verbose: bool = False) -> None:
+    """The CPython module. Without a host C++ compiler or Python's headers there is none (said on stderr): the C library is
+    whole, and the batch operators' Python calls say what is missing."""
+    for old in {MODULE, os.path.join(os.path.dirname(MODULE), "_batch.so")}:
+        if os.path.exists(old):
+            os.remove(old)                       # (it may not fit the library that was just built)
+    cxx, include = os.environ.get("CXX", "g++"), sysconfig.get_paths()["include"]
+    missing = f"the compiler {cxx}" if not shutil.which(cxx) else "Python.h" if not os.path.exists(os.path.join(include, "Python.h")) else None
+    if missing:
+        sys.stderr.write(f"{missing} is not there: {os.path.basename(MODULE)} (page_plan, page_put, page_attn and sample from Python) is not built\n")
+        return
+    tmp = MODULE + f".tmp{os.getpid()}"
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-I", include, "-o", tmp, os.path.join(HERE, "csrc", "py_batch.cpp")]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError(f"compiling {os.path.basename(MODULE)} failed")
+    os.replace(tmp, MODULE)
 
 
 if __name__ == "__main__":
