@@ -261,10 +261,12 @@ hipError_t launch_page_plan(const plan_args& a, hipStream_t s) {
     const long long want = ((long long)a.rows + 1023) / 1024;
     const int grid = want < 1 ? 1 : want > 1024 ? 1024 : (int)want;
     const size_t lds = 2 * ((size_t)a.n + 1) * sizeof(int);
-    // Four neighbouring rows a thread where requests add many: they mostly share their request and its page, looked up once
-    // (500 prompts: 8.3 us, 10.0 one by one); where they do not, four chains of loads one after the other (64 single rows:
-    // 6.9, 4.7 one by one)
-    if (a.rows / 8 >= a.n) k_page_plan<4><<<grid, PLAN_T, lds, s>>>(a);
+    // Four neighbouring rows a thread from as many rows on as two turns of a workgroup, whatever their requests: rows
+    // that share a request and its page look them up once, and threads have fewer bisections. Below, one row a thread: four
+    // chains of loads one after the other take longer than what they save. us one by one and by fours, at n x rows a request:
+    // 1 x 256 4.5 and 5.1, 8 x 32 4.9 and 5.6, 64 x 4 4.3 and 5.1, 500 x 1 6.5 and 7.4; 8 x 64 5.7 and 5.6, 64 x 8 5.3 and 5.1;
+    // 1 x 1024 6.2 and 5.2, 500 x 2 8.9 and 6.7, 64 x 64 8.3 and 6.1, 4000 x 1 20.5 and 18.4
+    if (a.rows >= 2 * PLAN_T) k_page_plan<4><<<grid, PLAN_T, lds, s>>>(a);
     else k_page_plan<1><<<grid, PLAN_T, lds, s>>>(a);
     return hipGetLastError();
 }

@@ -1061,3 +1061,21 @@ def test_first_step_beside_work_on_the_same_stream(tiny_model):
         b.step(7)
     side.synchronize()
     assert (x == count[0]).all(), "a replay repeats the other thread's work"
+
+
+@pytest.mark.parametrize("rows", [509, 511, 512, 513, 1027])
+def test_plan_row_counts_at_the_variants_border(ctx, rows):
+    """Rows on either side of where a thread takes four neighbouring ones, shared by requests of none to nine."""
+    rng = np.random.default_rng(rows)
+    add = rng.integers(0, 10, 2 * rows)
+    add = add[:int(np.searchsorted(np.cumsum(add), rows)) + 1]
+    add[-1] -= add.sum() - rows
+    n = len(add)
+    held = rng.integers(0, 60, n)
+    have, want = -(-held // 16), -(-(held + add) // 16)
+    ids = rng.permutation(int(want.sum()))
+    table, at = np.full((n, 5), -1), 0
+    for i in range(n):
+        table[i, :have[i]] = ids[at:at + have[i]]
+        at += have[i]
+    check_plan(ctx, held, add, 16, table, ids[at:], 0, rows, pos0=5)
