@@ -416,9 +416,10 @@ __global__ __launch_bounds__(256, waves_of(D, NTS, NTO)) void k_page_attn(pattn_
 }
 
 // One wave per (row, query head), or all four for many parts: lanes take four dimensions each, as many parts at once as
-// fit a wave. All four from 17 parts on: a wave alone reads them in turns that wait for each other (one request of 65521
-// positions, 32 heads: 7.5 us, a wave alone 20). With few parts the other waves only cost (256 requests of 32 heads: 7.3 us, four
-// waves 14; 48 of 16: 5.6 and 5.0).
+// fit a wave. All four from 17 parts on: a wave alone reads them in turns that wait for each other. With few parts the
+// other waves only cost. us a call of both kernels with one wave and with four, 32 heads of 64: one request 2 parts 8.3 and
+// 8.5, 8 parts 8.4 and 8.6, 12 parts 8.7 and 8.6, 16 parts 9.1 and 8.8, 32 parts 10.1 and 9.6, 128 parts 44 and 32; 8 requests
+// 4 parts 8.5 and 8.8, 16 parts 18.4 and 17.2; 256 requests of few parts: the join alone 7.3 and 14.
 template <class T, int D, bool MANY>
 __global__ __launch_bounds__(256) void k_page_join(pattn_args a) {
     constexpr int LP = D / 4, AT_ONCE = 64 / LP, WAVES = MANY ? 4 : 1;   // lanes per part, parts at once
@@ -525,8 +526,13 @@ bool page_attn_split(int D, bool single, pattn_args& a) {
     const long long own = own_tiles(a, nto, single), all = shared_tiles(a, col_groups(D, (long long)a.rows * a.grp));
     a.own_at = (a.prefix_len + 31) / 32 * 32;
     // Requests whose columns fill their workgroups read the shared positions themselves: sharing would not save reads,
-    // and nothing has to be joined (13 prompts of 300 rows behind 500 positions: 40 us, 138 apart). So do few requests with
-    // few shared positions (two behind 90: 9.6 us a call, 20.8 with parts and a join)
+    // and nothing has to be joined (13 prompts of 300 rows behind 500 positions: 40 us, 138 apart). us fused and apart for 16
+    // requests behind 1024 positions, 8 kv heads of 64: 16 rows each (own = 2 all) 22 and 28, 64 rows 26 and 57; 8 rows
+    // (own = 3 all) 24 and 17.
+    // So do few requests with few shared positions: own tiles times positions, one row each: 32 x 128 5.4 and 11.8, 4 x 1024
+    // 8.6 and 8.6, 16 x 256 8.4 and 12.5. Past 4096 it depends on the columns: with 16 a workgroup it pays up to about 32768
+    // (64 x 512 15.8 and 16.1, 64 x 1024 21.5 and 16.6), with 64 no longer at 6144 (16 requests of 8 rows behind 256: 15.6 and
+    // 14.1), so the bound is what holds for both
     a.fused = a.prefix_len == 0 || own <= all * 2 || own * a.prefix_len <= 4096;
     a.sp = a.pchunk = 0;
     if (!a.fused) {
