@@ -384,7 +384,8 @@ int sh_page_put(sh_ctx* ctx, const sh_page_shape* shape, int rows, const void* q
  * the gate. A row that sees nothing gives zeros and -inf. Keys of a page id outside [0, n_pages) count as not there. Rows
  * behind the last request's, and those past max_rows of their request, stay as they were. Weights are rounded to the
  * shape's type for their products with the values, sums are 32 bits: out is within half a place of the largest value seen
- * (and, where a single key outweighs a million others by 2^30, another quarter of one in f16).
+ * (and, where a single key outweighs a million others by 2^30, another quarter of one in f16). An infinite value whose
+ * weight rounds to 0 gives NaN; bf16 values beyond 2^88 may overflow the sums.
  * The shared positions are read once for the whole batch, as one matrix product for all rows. work: sh_page_attn_work's
  * bytes for the same sizes, on 256 bytes, the call's own until it is done (calls that may run at once, captured graphs
  * among them, need one each; nothing is kept in it between calls). */
