@@ -77,12 +77,17 @@ def build(verbose: bool = False) -> str:
 def build_module(verbose: bool = False) -> None:
     """The CPython module. Without a host C++ compiler or Python's headers there is none (said on stderr): the C library is
     whole, and the batch operators' Python calls say what is missing."""
-    for old in {MODULE, os.path.join(os.path.dirname(MODULE), "_batch.so")}:
-        if os.path.exists(old):
-            os.remove(old)                       # (it may not fit the library that was just built)
+    untagged = os.path.join(os.path.dirname(MODULE), "_batch.so")
+
+    def drop(*paths):
+        for old in paths:                        # (an earlier build's may not fit the library that was just built)
+            if os.path.exists(old):
+                os.remove(old)
+
     cxx, include = os.environ.get("CXX", "g++"), sysconfig.get_paths()["include"]
     missing = f"the compiler {cxx}" if not shutil.which(cxx) else "Python.h" if not os.path.exists(os.path.join(include, "Python.h")) else None
     if missing:
+        drop(untagged, MODULE)
         sys.stderr.write(f"{missing} is not there: {os.path.basename(MODULE)} (page_plan, page_put, page_attn and sample from Python) is not built\n")
         return
     tmp = MODULE + f".tmp{os.getpid()}"
@@ -91,9 +96,12 @@ def build_module(verbose: bool = False) -> None:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
+        drop(untagged, MODULE)
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError(f"compiling {os.path.basename(MODULE)} failed")
     os.replace(tmp, MODULE)
+    if untagged != MODULE:
+        drop(untagged)
 
 
 if __name__ == "__main__":
