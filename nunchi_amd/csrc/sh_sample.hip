@@ -289,7 +289,9 @@ template <int ST> struct row_search {
 #pragma unroll
             for (int e = 0; e < V; e++) own += w[e] = of(v[e], w0 + e);
             u64 before = found[2] + wave_scan(own) - own;
-            // (the block's sum is its words': one lane holds the target, at a word of some weight)
+            // The block's sum is its words': one lane holds the target, at a word of some weight. (Unless the row is written to
+            // meanwhile: then a word of the block, so that nothing is read outside the row)
+            if (lane == 0) found[3] = (u64)w0;
             if (before <= target && target < before + own) {
                 int e = 0;
                 while (before + w[e] <= target) before += w[e++];
