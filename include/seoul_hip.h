@@ -413,6 +413,74 @@ int sh_sample(sh_ctx* ctx, int rows, int vocab, const void* scores, long long ld
               const int32_t* top_k, const float* top_p, const float* min_p, const double* u, int32_t* ids, float* chance,
               void* work, size_t work_bytes);
 
+/* ---- drafted words: a step that tries a tree of words for each request ----
+ * A request's rows of the step (cu[i] .. cu[i + 1] - 1, as sh_page_plan's cu with add = its words) are its last word and words
+ * that someone drafted behind it: parent[row] is the place of the word before it among the request's rows (below the row's own
+ * place), or -1: the word before it is the last one held. sh_page_plan gives them slots, sh_tree_plan their positions and masks,
+ * sh_page_put writes them, sh_tree_attn is the attention, sh_sample picks a word for each row of scores, sh_tree_take finds the
+ * branch that the picks agree with and sh_page_keep moves its keys and values (once for each layer) to where the next step
+ * expects them. A request has at most 256 rows. Lengths, parents, masks, words and paths live on the device and are bounded
+ * there, as above. */
+
+/* Masks and positions of the rows. held[i], len[i]: positions of request i before the step and with its rows (sh_page_plan's held
+ * and len). mask [rows][ceil(max_rows / 32)]: bit k of a row is set when the request's k-th row is the row itself or a word that
+ * it follows; pos [rows]: pos0 + held + how many words it follows. A row whose parent, or a word that it follows, is not before
+ * it, and all rows of a request that was refused (len is not held + its rows), that has more than max_rows rows or rows past
+ * `rows`, get no bits and position -1: sh_page_put writes nothing for them and sh_tree_attn gives zeros. Rows behind the last
+ * request's stay as they were. max_rows 1 to 256. */
+int sh_tree_plan(sh_ctx* ctx, int n, int rows, const int32_t* cu, const int32_t* parent, const int32_t* held, const int32_t* len,
+                 int max_rows, uint32_t* mask, int32_t* pos, int pos0);
+
+/* sh_page_attn for trees: the last cu[i + 1] - cu[i] of a request's len[i] positions are its rows' words. A row sees the shared
+ * positions, its request's own before those words, and of the words those whose bits its mask has (its own bit set); its
+ * position is that of the last own one before the words plus its bits, and the shape's window counts by it. A row without its
+ * own bit sees nothing: zeros and -inf. Masks need not come from sh_tree_plan: any bits of the request's words are followed.
+ * All else, work memory among it (sh_tree_attn_work), is as sh_page_attn says. max_rows 1 to 256; masks have
+ * ceil(max_rows / 32) words a row. */
+int sh_tree_attn_work(const sh_page_shape* shape, int n, int rows, int max_rows, int prefix_len, int max_len, size_t* bytes);
+int sh_tree_attn(sh_ctx* ctx, const sh_page_shape* shape, int n, int rows, const int32_t* cu, int max_rows, const uint32_t* mask,
+                 const void* q, const void* keys, const void* values, const int32_t* prefix, int prefix_len,
+                 const int32_t* table, int cols, const int32_t* len, int max_len, const float* gate, void* out, float* lse,
+                 void* work, size_t work_bytes);
+
+/* How likely words are: of each row of scores [rows][vocab] (type and ld as sh_sample's), with z = (score - max) / temp and
+ * L = sum of e^z,
+ *   logp      [rows][n_words]  z - log L of the words words[rows][n_words] (n_words 0: none)
+ *   entropy   [rows]           -sum of p log p, p = e^z / L (null: none)
+ *   top_words, top_logp [rows][n_top]  the n_top likeliest words, by score and, among equal ones, by index, and their log
+ *                              probabilities (either may be null; n_top 0 to 64)
+ * temp is one value per row or null (1). temp 0 is sh_sample's greedy row: the first of the largest scores has log probability
+ * 0, all others -inf; a negative or NaN temp gives NaN. Scores of -inf or NaN have log probability -inf and are not among the
+ * likeliest (-1 and -inf where too few are left); a score of +inf shares everything with its like. Words outside [0, vocab)
+ * have -inf. A row with nothing above -inf has entropy 0. vocab at most 524288. work: sh_word_probs_work's bytes, as above. */
+int sh_word_probs_work(int rows, int vocab, int n_top, size_t* bytes);
+int sh_word_probs(sh_ctx* ctx, int rows, int vocab, const void* scores, long long ld, int type, const float* temp,
+                  const int32_t* words, int n_words, float* logp, float* entropy, int32_t* top_words, float* top_logp,
+                  int n_top, void* work, size_t work_bytes);
+
+/* The branch of each request that its picks agree with: row 0 is kept; while the pick after a kept row (picks[row], a word) is
+ * the word of one of its children (words[row]), the first such child is kept too.
+ *   path    [rows]  at the request's j-th row the place of the j-th kept row among the request's rows; -1 behind them
+ *   count   [n]     kept rows
+ *   next    [n]     the pick after the last kept row: the word that the next step starts with (-1 where there is none)
+ *   len_out [n]     held + count
+ * Picks below 0 agree with nothing. A request without rows keeps its length; one that was refused (as above) keeps nothing, its
+ * len_out is len. With table [n][cols] (null: not done) the pages between ceil(len_out / page) and ceil(len / page) of each
+ * request go back, in the order of the requests: *taken of free_pages [n_free] were given out (sh_page_plan's taken_out),
+ * *taken_out is that less the pages that go back, which are written from free_pages[*taken_out] on; pages past *taken are not
+ * written. n up to 4096. */
+int sh_tree_take(sh_ctx* ctx, int n, int rows, const int32_t* cu, const int32_t* parent, const int32_t* words,
+                 const int32_t* picks, const int32_t* held, const int32_t* len, int32_t* path, int32_t* count, int32_t* next,
+                 int32_t* len_out, int page, const int32_t* table, int cols, int32_t* free_pages, int n_free,
+                 const int32_t* taken, int32_t* taken_out);
+
+/* Keys and values of the kept rows of one layer moved, in place: with base = len[i] - the request's rows, position
+ * base + path[j] to base + j, j in order, for every j of the request's rows with j < path[j] < rows; other entries move nothing.
+ * len is the length with the step's rows. Places in pages outside [0, n_pages), past `cols` or before the request's first
+ * position move nothing either. No two requests may have a page of such positions in common. */
+int sh_page_keep(sh_ctx* ctx, const sh_page_shape* shape, int n, int rows, const int32_t* cu, const int32_t* path,
+                 const int32_t* len, const int32_t* table, int cols, void* keys, void* values);
+
 /* Synchronise the context's stream (for callers of the _dev entry points). */
 int sh_sync(sh_ctx* ctx);
 

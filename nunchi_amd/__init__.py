@@ -32,6 +32,7 @@ EXPORTS = [
     "sh_ears_load", "sh_ears_free", "sh_ears_info", "sh_ears_positions", "sh_ears_encode", "sh_ears_mel",
     "sh_bench_empty", "sh_bench_read", "sh_bench_xcc", "sh_bench_l2_reuse",
     "sh_page_plan", "sh_page_put", "sh_page_attn_work", "sh_page_attn", "sh_sample_work", "sh_sample",
+    "sh_tree_plan", "sh_tree_attn_work", "sh_tree_attn", "sh_word_probs_work", "sh_word_probs", "sh_tree_take", "sh_page_keep",
 ]
 
 
@@ -161,6 +162,13 @@ def load_library(path: str = LIB_PATH):
         "sh_page_attn": (i, [vp, vp, i, i, vp, i, vp, vp, vp, vp, i, vp, i, vp, i, vp, vp, vp, vp, C.c_size_t]),
         "sh_sample_work": (i, [i, i, P(C.c_size_t)]),
         "sh_sample": (i, [vp, i, i, vp, C.c_longlong, i, vp, vp, vp, vp, vp, vp, vp, vp, C.c_size_t]),
+        "sh_tree_plan": (i, [vp, i, i, vp, vp, vp, vp, i, vp, vp, i]),
+        "sh_tree_attn_work": (i, [vp, i, i, i, i, i, P(C.c_size_t)]),
+        "sh_tree_attn": (i, [vp, vp, i, i, vp, i, vp, vp, vp, vp, vp, i, vp, i, vp, i, vp, vp, vp, vp, C.c_size_t]),
+        "sh_word_probs_work": (i, [i, i, i, P(C.c_size_t)]),
+        "sh_word_probs": (i, [vp, i, i, vp, C.c_longlong, i, vp, vp, i, vp, vp, vp, vp, i, vp, C.c_size_t]),
+        "sh_tree_take": (i, [vp, i, i, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i, vp, i, vp, i, vp, vp]),
+        "sh_page_keep": (i, [vp, vp, i, i, vp, vp, vp, vp, i, vp, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -737,7 +745,8 @@ class Voice:
         return picks[:u.size], keep[:u.size]
 
 
-from .batch import (PageShape, page_attn, page_attn_work, page_plan, page_put, sample, sample_work)  # noqa: E402
+from .batch import (PageShape, page_attn, page_attn_work, page_keep, page_plan, page_put, sample, sample_work, tree_attn,  # noqa: E402
+                    tree_attn_work, tree_plan, tree_take, word_probs, word_probs_work)
 
 
 @atexit.register

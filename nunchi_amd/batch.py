@@ -1,6 +1,8 @@
 """Operators that serve a batch of conversations, on device tensors: pages of keys and values with their block tables and
 slot maps (page_plan), the write of a step's positions (page_put), attention over a shared prefix and each conversation's
-own pages (page_attn), and the next words (sample). include/seoul_hip.h says what each computes.
+own pages (page_attn), and the next words (sample). For steps that try drafted words: their masks and positions (tree_plan),
+attention over trees of them (tree_attn), how likely words are (word_probs), the branch that is kept (tree_take) and its moves
+(page_keep). include/seoul_hip.h says what each computes.
 
 Tensors are torch's, or anything with its data_ptr, dtype, shape, is_contiguous and get_device; they are contiguous and on
 the context's device. Calls are enqueued on the context's stream and do not wait, so a context made on the stream that the
@@ -13,7 +15,8 @@ import ctypes as C
 import nunchi_amd as _n
 
 _TYPES = {"f16": 1, "bf16": 30}
-_native = None      # (the module, addresses of the four entry points): made by the first call
+_ENTRIES = ("sh_page_plan", "sh_page_put", "sh_page_attn", "sh_sample", "sh_tree_plan", "sh_tree_attn", "sh_word_probs", "sh_tree_take", "sh_page_keep")
+_native = None      # (the module, addresses of _ENTRIES): made by the first call
 
 
 def _load():
@@ -23,7 +26,7 @@ def _load():
     except ImportError as e:
         raise ImportError("nunchi_amd._batch is not built for this Python: run `python -m nunchi_amd.build` (it needs a C++ compiler and Python.h)") from e
     lib = _n.load_library()
-    _native = (_batch, *(C.cast(getattr(lib, f), C.c_void_p).value for f in ("sh_page_plan", "sh_page_put", "sh_page_attn", "sh_sample")))
+    _native = (_batch, *(C.cast(getattr(lib, f), C.c_void_p).value for f in _ENTRIES))
     return _native
 
 
@@ -98,5 +101,70 @@ def sample(ctx, scores, u, ids, work, temp=None, top_k=None, top_p=None, min_p=N
     min_p f32 and top_k i32, [rows] or None; ids [rows] i32 and chance [rows] f32 out; work u8 of sample_work's bytes."""
     native = _native or _load()
     rc = native[0].sample(native[4], ctx.h.value, ctx.device, scores, u, ids, work, temp, top_k, top_p, min_p, chance)
+    if rc:
+        _n._check(rc)
+
+
+def tree_plan(ctx, cu, parent, held, length, mask, pos, max_rows: int, pos0: int = 0):
+    """Masks and positions of drafted words (sh_tree_plan): cu [n + 1], parent [rows], held and length [n] i32 in;
+    mask [rows][ceil(max_rows / 32)] i32 (its bits) and pos [rows] i32 out."""
+    native = _native or _load()
+    rc = native[0].tree_plan(native[5], ctx.h.value, ctx.device, cu, parent, held, length, mask, pos, max_rows, pos0)
+    if rc:
+        _n._check(rc)
+
+
+def tree_attn_work(shape: PageShape, n: int, rows: int, max_len: int, max_rows: int, prefix_len: int = 0) -> int:
+    """Bytes of work memory of a tree_attn call of these sizes."""
+    size = C.c_size_t()
+    _n._check(_n.load_library().sh_tree_attn_work(C.byref(shape), int(n), int(rows), int(max_rows), int(prefix_len), int(max_len), C.byref(size)))
+    return size.value
+
+
+def tree_attn(ctx, shape: PageShape, q, keys, values, table, length, cu, mask, out, work, max_len: int, max_rows: int, prefix=None,
+              prefix_len: int = 0, gate=None, lse=None):
+    """Attention of trees of drafted words over the shared prefix, each request's own pages and the words before them
+    (sh_tree_attn): cu [n + 1] i32 and tree_plan's mask, the others as page_attn's, work u8 of tree_attn_work's bytes."""
+    native = _native or _load()
+    rc = native[0].tree_attn(native[6], ctx.h.value, ctx.device, shape.address, q, keys, values, table, length, cu, mask, out, work, max_len, max_rows,
+                             prefix, prefix_len, gate, lse)
+    if rc:
+        _n._check(rc)
+
+
+def word_probs_work(rows: int, vocab: int, n_top: int = 0) -> int:
+    """Bytes of work memory of a word_probs call of these sizes."""
+    size = C.c_size_t()
+    _n._check(_n.load_library().sh_word_probs_work(int(rows), int(vocab), int(n_top), C.byref(size)))
+    return size.value
+
+
+def word_probs(ctx, scores, work, temp=None, words=None, logp=None, entropy=None, top_words=None, top_logp=None):
+    """How likely words are (sh_word_probs): scores [rows][vocab] in f32, f16 or bf16, temp [rows] f32 or None (1), words
+    [rows][m] i32 in; logp [rows][m], entropy [rows], top_logp [rows][k] f32 and top_words [rows][k] i32 (k up to 64) out,
+    each or None; work u8 of word_probs_work's bytes."""
+    native = _native or _load()
+    rc = native[0].word_probs(native[7], ctx.h.value, ctx.device, scores, work, temp, words, logp, entropy, top_words, top_logp)
+    if rc:
+        _n._check(rc)
+
+
+def tree_take(ctx, cu, parent, words, picks, held, length, path, count, next, length_out, table=None, page: int = 16, free=None, taken=None,
+              taken_out=None):
+    """The branch of drafted words that the picks agree with (sh_tree_take): cu [n + 1], parent, words and picks [rows], held
+    and length [n] i32 in; path [rows], count, next and length_out [n] i32 out. With table [n][cols] i32 the pages behind the
+    new lengths go back to free [n_free] i32, taken [1] i32 in and taken_out [1] out."""
+    native = _native or _load()
+    rc = native[0].tree_take(native[8], ctx.h.value, ctx.device, cu, parent, words, picks, held, length, path, count, next, length_out, table, page, free,
+                             taken, taken_out)
+    if rc:
+        _n._check(rc)
+
+
+def page_keep(ctx, shape: PageShape, cu, path, length, table, keys, values):
+    """Keys and values of the kept branch moved to where the next step expects them, in one layer (sh_page_keep): cu [n + 1],
+    tree_take's path [rows], length [n] (with the step's rows) and table [n][cols] i32."""
+    native = _native or _load()
+    rc = native[0].page_keep(native[9], ctx.h.value, ctx.device, shape.address, cu, path, length, table, keys, values)
     if rc:
         _n._check(rc)

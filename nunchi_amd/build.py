@@ -22,6 +22,7 @@ LIB = os.path.join(HERE, "libseoul_hip.so")
 MODULE = os.path.join(HERE, "_batch" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 SOURCES = ["csrc/sh_kernels.hip", "csrc/sh_voice.hip", "csrc/sh_prefill.hip", "csrc/sh_noalloc.hip", "csrc/sh_codec.hip",
            "csrc/sh_ears.hip", "csrc/sh_calib.hip", "csrc/sh_pages.hip", "csrc/sh_page_attn.hip", "csrc/sh_sample.hip",
+           "csrc/sh_tree.hip", "csrc/sh_tree_attn.hip", "csrc/sh_word_probs.hip",
            "csrc/sh_engine.cpp", "csrc/sh_codec_host.cpp", "csrc/sh_ears_host.cpp", "csrc/sh_voice_host.cpp",
            "csrc/sh_prefill_host.cpp", "csrc/sh_serve_host.cpp", "csrc/gguf_file.cpp", "csrc/sh_file.cpp"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

@@ -250,11 +250,152 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                               (const float*)top_p.p, (const float*)min_p.p, (const double*)u.p, (int32_t*)ids.p, (float*)chance.p, work.p, (size_t)work.d[0]));
 }
 
+// rows of a step in packed order: cu [n + 1] and so many rows
+bool packed(const tensor& cu, const tensor& rows, const char* name) {
+    if (!dims(cu, "cu", 1) || !dims(rows, name, 1) || !fits(cu, "cu") || !fits(rows, name)) return false;
+    if (cu.d[0] >= 2) return true;
+    PyErr_SetString(PyExc_ValueError, "cu has fewer than 2 entries");
+    return false;
+}
+
+PyObject* tree_plan(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    decltype(&sh_tree_plan) fn;
+    sh_ctx* ctx;
+    long dev;
+    if (!head(a, n_args, 11, fn, ctx, dev)) return nullptr;
+    tensor cu, parent, held, length, mask, pos;
+    long long max_rows, pos0;
+    if (!read(a[3], "cu", dev, K_I32, cu) || !read(a[4], "parent", dev, K_I32, parent) || !read(a[5], "held", dev, K_I32, held) ||
+        !read(a[6], "length", dev, K_I32, length) || !read(a[7], "mask", dev, K_I32, mask) || !read(a[8], "pos", dev, K_I32, pos) ||
+        !number(a[9], 1, 256, "max_rows", max_rows) || !number(a[10], I32_MIN, I32_MAX, "pos0", pos0))
+        return nullptr;
+    if (!packed(cu, parent, "parent")) return nullptr;
+    const long long n = cu.d[0] - 1, rows = parent.d[0];
+    if (!has(held, "held", 1, n) || !has(length, "length", 1, n) || !has(mask, "mask", 2, rows, (max_rows + 31) / 32) || !has(pos, "pos", 1, rows)) return nullptr;
+    return PyLong_FromLong(fn(ctx, (int)n, (int)rows, (const int32_t*)cu.p, (const int32_t*)parent.p, (const int32_t*)held.p, (const int32_t*)length.p,
+                              (int)max_rows, (uint32_t*)mask.p, (int32_t*)pos.p, (int)pos0));
+}
+
+PyObject* tree_attn(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    decltype(&sh_tree_attn) fn;
+    sh_ctx* ctx;
+    long dev;
+    if (!head(a, n_args, 19, fn, ctx, dev)) return nullptr;
+    const sh_page_shape* s = shape_of(a[3]);
+    if (!s) return nullptr;
+    const int kind = kind_for(s->type);
+    tensor q, keys, values, table, length, cu, mask, out, work, prefix, gate, lse;
+    long long max_len, max_rows, prefix_len;
+    if (!read(a[4], "q", dev, kind, q) || !read(a[5], "keys", dev, kind, keys) || !read(a[6], "values", dev, kind, values) ||
+        !read(a[7], "table", dev, K_I32, table) || !read(a[8], "length", dev, K_I32, length) || !read(a[9], "cu", dev, K_I32, cu) ||
+        !read(a[10], "mask", dev, K_I32, mask) || !read(a[11], "out", dev, kind, out) || !read(a[12], "work", dev, K_U8, work) ||
+        !number(a[13], I32_MIN, I32_MAX, "max_len", max_len) || !number(a[14], 1, 256, "max_rows", max_rows) ||
+        !number(a[16], I32_MIN, I32_MAX, "prefix_len", prefix_len) || (prefix_len && !read(a[15], "prefix", dev, K_I32, prefix)) ||
+        !read(a[17], "gate", dev, K_F32, gate) || !read(a[18], "lse", dev, K_F32, lse))
+        return nullptr;
+    if (!dims(q, "q", 3) || !dims(length, "length", 1) || !dims(table, "table", 2) || !dims(work, "work", 1) || !fits(q, "q") || !fits(length, "length") ||
+        !fits(table, "table"))
+        return nullptr;
+    const long long rows = q.d[0], n = length.d[0], H = s->n_head, D = s->head_dim;
+    if (!has(q, "q", 3, rows, H, D) || !has(keys, "keys", 4, s->n_pages, s->n_kv, s->page, D) || !has(values, "values", 4, s->n_pages, s->n_kv, s->page, D) ||
+        !has(table, "table", 2, n, table.d[1]) || !has(out, "out", 3, rows, H, D) || !has(cu, "cu", 1, n + 1) ||
+        !has(mask, "mask", 2, rows, (max_rows + 31) / 32) || !has(gate, "gate", 2, rows, H, 0, 0, true) || !has(lse, "lse", 2, rows, H, 0, 0, true))
+        return nullptr;
+    if (prefix_len > 0 && (!dims(prefix, "prefix", 1) || prefix.d[0] * s->page < prefix_len)) {
+        if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "prefix has fewer pages than prefix_len needs");
+        return nullptr;
+    }
+    return PyLong_FromLong(fn(ctx, s, (int)n, (int)rows, (const int32_t*)cu.p, (int)max_rows, (const uint32_t*)mask.p, q.p, keys.p, values.p,
+                              (const int32_t*)prefix.p, (int)prefix_len, (const int32_t*)table.p, (int)table.d[1], (const int32_t*)length.p, (int)max_len,
+                              (const float*)gate.p, out.p, (float*)lse.p, work.p, (size_t)work.d[0]));
+}
+
+PyObject* word_probs(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    decltype(&sh_word_probs) fn;
+    sh_ctx* ctx;
+    long dev;
+    if (!head(a, n_args, 11, fn, ctx, dev)) return nullptr;
+    tensor scores, work, temp, words, logp, entropy, top_words, top_logp;
+    if (!read(a[3], "scores", dev, K_F32 | K_F16 | K_BF16, scores) || !read(a[4], "work", dev, K_U8, work) || !read(a[5], "temp", dev, K_F32, temp) ||
+        !read(a[6], "words", dev, K_I32, words) || !read(a[7], "logp", dev, K_F32, logp) || !read(a[8], "entropy", dev, K_F32, entropy) ||
+        !read(a[9], "top_words", dev, K_I32, top_words) || !read(a[10], "top_logp", dev, K_F32, top_logp))
+        return nullptr;
+    if (!dims(scores, "scores", 2) || !dims(work, "work", 1) || !fits(scores, "scores")) return nullptr;
+    if ((!words.none() && (!dims(words, "words", 2) || !fits(words, "words"))) || (!top_words.none() && (!dims(top_words, "top_words", 2) || !fits(top_words, "top_words"))) ||
+        (!top_logp.none() && (!dims(top_logp, "top_logp", 2) || !fits(top_logp, "top_logp"))))
+        return nullptr;
+    const long long rows = scores.d[0], vocab = scores.d[1], n_words = words.none() ? 0 : words.d[1];
+    const long long n_top = !top_words.none() ? top_words.d[1] : !top_logp.none() ? top_logp.d[1] : 0;
+    if (words.none() != logp.none()) {
+        PyErr_SetString(PyExc_ValueError, "words and logp go together");
+        return nullptr;
+    }
+    if (!has(temp, "temp", 1, rows, 0, 0, 0, true) || !has(words, "words", 2, rows, n_words, 0, 0, true) || !has(logp, "logp", 2, rows, n_words, 0, 0, true) ||
+        !has(entropy, "entropy", 1, rows, 0, 0, 0, true) || !has(top_words, "top_words", 2, rows, n_top, 0, 0, true) ||
+        !has(top_logp, "top_logp", 2, rows, n_top, 0, 0, true))
+        return nullptr;
+    return PyLong_FromLong(fn(ctx, (int)rows, (int)vocab, scores.p, vocab, type_of(scores.kind), (const float*)temp.p, (const int32_t*)words.p, (int)n_words,
+                              (float*)logp.p, (float*)entropy.p, (int32_t*)top_words.p, (float*)top_logp.p, (int)n_top, work.p, (size_t)work.d[0]));
+}
+
+PyObject* tree_take(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    decltype(&sh_tree_take) fn;
+    sh_ctx* ctx;
+    long dev;
+    if (!head(a, n_args, 18, fn, ctx, dev)) return nullptr;
+    tensor cu, parent, words, picks, held, length, path, count, next, length_out, table, free_pages, taken, taken_out;
+    long long page;
+    if (!read(a[3], "cu", dev, K_I32, cu) || !read(a[4], "parent", dev, K_I32, parent) || !read(a[5], "words", dev, K_I32, words) ||
+        !read(a[6], "picks", dev, K_I32, picks) || !read(a[7], "held", dev, K_I32, held) || !read(a[8], "length", dev, K_I32, length) ||
+        !read(a[9], "path", dev, K_I32, path) || !read(a[10], "count", dev, K_I32, count) || !read(a[11], "next", dev, K_I32, next) ||
+        !read(a[12], "length_out", dev, K_I32, length_out) || !read(a[13], "table", dev, K_I32, table) || !number(a[14], I32_MIN, I32_MAX, "page", page) ||
+        !read(a[15], "free", dev, K_I32, free_pages) || !read(a[16], "taken", dev, K_I32, taken) || !read(a[17], "taken_out", dev, K_I32, taken_out))
+        return nullptr;
+    if (!packed(cu, parent, "parent")) return nullptr;
+    const long long n = cu.d[0] - 1, rows = parent.d[0];
+    if (!has(words, "words", 1, rows) || !has(picks, "picks", 1, rows) || !has(held, "held", 1, n) || !has(length, "length", 1, n) || !has(path, "path", 1, rows) ||
+        !has(count, "count", 1, n) || !has(next, "next", 1, n) || !has(length_out, "length_out", 1, n))
+        return nullptr;
+    if (!table.none() && (!dims(table, "table", 2) || !fits(table, "table") || !has(table, "table", 2, n, table.d[1]) || !dims(free_pages, "free", 1) ||
+                          !fits(free_pages, "free") || !has(taken, "taken", 1, 1) || !has(taken_out, "taken_out", 1, 1)))
+        return nullptr;
+    return PyLong_FromLong(fn(ctx, (int)n, (int)rows, (const int32_t*)cu.p, (const int32_t*)parent.p, (const int32_t*)words.p, (const int32_t*)picks.p,
+                              (const int32_t*)held.p, (const int32_t*)length.p, (int32_t*)path.p, (int32_t*)count.p, (int32_t*)next.p, (int32_t*)length_out.p,
+                              (int)page, (const int32_t*)table.p, (int)table.d[1], (int32_t*)free_pages.p, (int)free_pages.d[0], (const int32_t*)taken.p,
+                              (int32_t*)taken_out.p));
+}
+
+PyObject* page_keep(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    decltype(&sh_page_keep) fn;
+    sh_ctx* ctx;
+    long dev;
+    if (!head(a, n_args, 10, fn, ctx, dev)) return nullptr;
+    const sh_page_shape* s = shape_of(a[3]);
+    if (!s) return nullptr;
+    const int kind = kind_for(s->type);
+    tensor cu, path, length, table, keys, values;
+    if (!read(a[4], "cu", dev, K_I32, cu) || !read(a[5], "path", dev, K_I32, path) || !read(a[6], "length", dev, K_I32, length) ||
+        !read(a[7], "table", dev, K_I32, table) || !read(a[8], "keys", dev, kind, keys) || !read(a[9], "values", dev, kind, values))
+        return nullptr;
+    if (!packed(cu, path, "path") || !dims(table, "table", 2) || !fits(table, "table")) return nullptr;
+    const long long n = cu.d[0] - 1, rows = path.d[0], D = s->head_dim;
+    if (!has(length, "length", 1, n) || !has(table, "table", 2, n, table.d[1]) || !has(keys, "keys", 4, s->n_pages, s->n_kv, s->page, D) ||
+        !has(values, "values", 4, s->n_pages, s->n_kv, s->page, D))
+        return nullptr;
+    return PyLong_FromLong(fn(ctx, s, (int)n, (int)rows, (const int32_t*)cu.p, (const int32_t*)path.p, (const int32_t*)length.p, (const int32_t*)table.p,
+                              (int)table.d[1], keys.p, values.p));
+}
+
 PyMethodDef methods[] = {
     {"page_plan", (PyCFunction)(void (*)())page_plan, METH_FASTCALL, nullptr},
     {"page_put", (PyCFunction)(void (*)())page_put, METH_FASTCALL, nullptr},
     {"page_attn", (PyCFunction)(void (*)())page_attn, METH_FASTCALL, nullptr},
     {"sample", (PyCFunction)(void (*)())sample, METH_FASTCALL, nullptr},
+    {"tree_plan", (PyCFunction)(void (*)())tree_plan, METH_FASTCALL, nullptr},
+    {"tree_attn", (PyCFunction)(void (*)())tree_attn, METH_FASTCALL, nullptr},
+    {"word_probs", (PyCFunction)(void (*)())word_probs, METH_FASTCALL, nullptr},
+    {"tree_take", (PyCFunction)(void (*)())tree_take, METH_FASTCALL, nullptr},
+    {"page_keep", (PyCFunction)(void (*)())page_keep, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_batch", "Calls of the batch operators on device tensors.", -1, methods, nullptr, nullptr, nullptr, nullptr};

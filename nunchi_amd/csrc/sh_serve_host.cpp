@@ -104,6 +104,26 @@ void attn_work(const pattn_args& a, int D, size_t* sums, size_t* all) {
     *sums = align256(parts * D * sizeof(float));
     *all = *sums + align256(parts * sizeof(float2));
 }
+
+// sizes of a call over scores into its argument block (its parts among them); null when they are in range
+const char* probs_sizes(int rows, int vocab, int n_top, probs_args& a) {
+    if (rows < 0 || vocab < 1 || vocab > SAMPLE_MAX_VOCAB) return "rows is negative, or vocab not 1 to 524288";
+    if (n_top < 0 || n_top > PROBS_MAX_TOP) return "n_top must be 0 to 64";
+    a.rows = rows;
+    a.vocab = vocab;
+    a.n_top = n_top;
+    word_probs_split(a);
+    if ((long long)rows * a.parts > most_blocks(256)) return "more rows than one launch holds";
+    return nullptr;
+}
+
+// bytes of the parts' sums, and behind them of their likeliest words
+void probs_work(const probs_args& a, size_t* sums, size_t* all) {
+    const size_t parts = (size_t)a.rows * a.parts;
+    *sums = align256(parts * sizeof(probs_part));
+    *all = *sums + align256(parts * (a.n_top > 0 ? a.n_top : 1) * sizeof(word_score));
+    if (*all < 256) *all = 256;
+}
 }  // namespace
 
 #define SH_ENTRY try {
@@ -305,6 +325,225 @@ int sh_sample(sh_ctx* c, int rows, int vocab, const void* scores, long long ld, 
     a.ids = ids;
     a.chance = chance;
     return done(launch_sample(a, c->stream), who);
+    SH_ENTRY_END
+}
+
+int sh_tree_plan(sh_ctx* c, int n, int rows, const int32_t* cu, const int32_t* parent, const int32_t* held, const int32_t* len, int max_rows,
+                 uint32_t* mask, int32_t* pos, int pos0) {
+    SH_ENTRY
+    const char* who = "sh_tree_plan";
+    if (!c || n < 1 || rows < 0 || pos0 < 0) return bad(who, "null context, n below 1, or a size is negative");
+    if (n > most_blocks(TREE_MAX)) return bad(who, "more requests than one launch holds");
+    if (max_rows < 1 || max_rows > TREE_MAX) return bad(who, "max_rows must be 1 to 256");
+    if (rows == 0) return SH_OK;
+    if (!cu || !parent || !held || !len || !mask || !pos) return bad(who, "null");
+    const size_t each = (size_t)n * 4, row4 = (size_t)rows * 4;
+    const int words = (max_rows + 31) / 32;
+    const extent in[] = {{cu, each + 4}, {parent, row4}, {held, each}, {len, each}}, out[] = {{mask, row4 * words}, {pos, row4}};
+    if (const char* f = overlap(in, out)) return bad(who, f);
+    const on_device dev(c->device);
+    if (dev.e != hipSuccess) return done(dev.e, who);
+    tree_plan_args a{};
+    a.n = n;
+    a.rows = rows;
+    a.max_rows = max_rows;
+    a.words = words;
+    a.pos0 = pos0;
+    a.cu = cu;
+    a.parent = parent;
+    a.held = held;
+    a.len = len;
+    a.mask = mask;
+    a.pos = pos;
+    return done(launch_tree_plan(a, c->stream), who);
+    SH_ENTRY_END
+}
+
+int sh_tree_attn_work(const sh_page_shape* s, int n, int rows, int max_rows, int prefix_len, int max_len, size_t* bytes) {
+    SH_ENTRY
+    const char* who = "sh_tree_attn_work";
+    if (!bytes) return bad(who, "null");
+    *bytes = 0;
+    if (max_rows > TREE_MAX) return bad(who, "max_rows must be 1 to 256");
+    pattn_args a{};
+    if (const char* f = attn_sizes(s, n, rows, max_rows, prefix_len, max_len, false, a)) return bad(who, f);
+    size_t sums;
+    attn_work(a, s->head_dim, &sums, bytes);
+    if (*bytes < 256) *bytes = 256;
+    return SH_OK;
+    SH_ENTRY_END
+}
+
+int sh_tree_attn(sh_ctx* c, const sh_page_shape* s, int n, int rows, const int32_t* cu, int max_rows, const uint32_t* mask, const void* q, const void* keys,
+                 const void* values, const int32_t* prefix, int prefix_len, const int32_t* table, int cols, const int32_t* len, int max_len,
+                 const float* gate, void* out, float* lse, void* work, size_t work_bytes) {
+    SH_ENTRY
+    const char* who = "sh_tree_attn";
+    if (max_rows > TREE_MAX) return bad(who, "max_rows must be 1 to 256");
+    pattn_args a{};
+    if (const char* f = attn_sizes(s, n, rows, max_rows, prefix_len, max_len, false, a)) return bad(who, f);
+    if (!c) return bad(who, "null context");
+    if (rows == 0) return SH_OK;
+    if (!cu || !mask || !q || !keys || !values || !len || !out || (prefix_len && !prefix) || cols < 0 || (cols && !table)) return bad(who, "null, or cols negative");
+    if (off(q, 16) || off(keys, 16) || off(values, 16) || off(out, 16)) return bad(who, "queries, keys, values and outputs start on 16 bytes");
+    size_t sums, all;
+    attn_work(a, s->head_dim, &sums, &all);
+    if (all && (!work || work_bytes < all || off(work, 256))) return bad(who, "work is missing, smaller than sh_tree_attn_work says, or not on 256 bytes");
+    const int words = (max_rows + 31) / 32;
+    const size_t q_bytes = (size_t)rows * s->n_head * s->head_dim * 2, rh = (size_t)rows * s->n_head * sizeof(float),
+                 cache = (size_t)s->n_pages * s->n_kv * s->page * s->head_dim * 2;
+    const extent in[] = {{q, q_bytes}, {keys, cache}, {values, cache}, {gate, rh}, {len, (size_t)n * 4}, {table, (size_t)n * cols * 4}, {cu, ((size_t)n + 1) * 4},
+                         {prefix, ((size_t)prefix_len + s->page - 1) / s->page * 4}, {mask, (size_t)rows * words * 4}},
+                 to[] = {{out, q_bytes}, {lse, rh}, {work, all}};
+    if (const char* f = overlap(in, to)) return bad(who, f);
+    const on_device dev(c->device);
+    if (dev.e != hipSuccess) return done(dev.e, who);
+    a.cols = cols;
+    a.cu = cu;
+    a.prefix = prefix;
+    a.table = table;
+    a.len = len;
+    a.q = q;
+    a.keys = keys;
+    a.values = values;
+    a.gate = gate;
+    a.out = out;
+    a.lse = lse;
+    a.part_o = static_cast<float*>(work);
+    a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(work) + sums);
+    a.mask = mask;
+    a.words = words;
+    return done(launch_tree_attn(s->head_dim, s->type, a, c->stream), who);
+    SH_ENTRY_END
+}
+
+int sh_word_probs_work(int rows, int vocab, int n_top, size_t* bytes) {
+    SH_ENTRY
+    if (!bytes) return bad("sh_word_probs_work", "null");
+    *bytes = 0;
+    probs_args a{};
+    if (const char* f = probs_sizes(rows, vocab, n_top, a)) return bad("sh_word_probs_work", f);
+    size_t sums;
+    probs_work(a, &sums, bytes);
+    return SH_OK;
+    SH_ENTRY_END
+}
+
+int sh_word_probs(sh_ctx* c, int rows, int vocab, const void* scores, long long ld, int type, const float* temp, const int32_t* words, int n_words,
+                  float* logp, float* entropy, int32_t* top_words, float* top_logp, int n_top, void* work, size_t work_bytes) {
+    SH_ENTRY
+    const char* who = "sh_word_probs";
+    probs_args a{};
+    if (!c) return bad(who, "null context");
+    if (const char* f = probs_sizes(rows, vocab, n_top, a)) return bad(who, f);
+    if (n_words < 0) return bad(who, "n_words is negative");
+    if (rows == 0) return SH_OK;
+    if (!scores || (n_words && (!words || !logp)) || (n_top && !top_words && !top_logp)) return bad(who, "null");
+    if (type != SH_F32 && !is_16(type)) return bad(who, "type must be SH_F32, SH_F16 or SH_BF16");
+    if (ld < vocab) return bad(who, "a row (ld) is shorter than vocab");
+    if (off(scores, type == SH_F32 ? 4 : 2)) return bad(who, "scores are not aligned to their type");
+    size_t sums, all;
+    probs_work(a, &sums, &all);
+    if (!work || work_bytes < all || off(work, 256)) return bad(who, "work is missing, smaller than sh_word_probs_work says, or not on 256 bytes");
+    const size_t each = (size_t)rows * 4;
+    const extent in[] = {{scores, ((size_t)(rows - 1) * ld + vocab) * (type == SH_F32 ? 4 : 2)}, {temp, each}, {n_words ? words : nullptr, each * n_words}},
+                 out[] = {{n_words ? logp : nullptr, each * n_words}, {entropy, each}, {n_top ? top_words : nullptr, each * n_top},
+                          {n_top ? top_logp : nullptr, each * n_top}, {work, all}};
+    if (const char* f = overlap(in, out)) return bad(who, f);
+    const on_device dev(c->device);
+    if (dev.e != hipSuccess) return done(dev.e, who);
+    a.type = type;
+    a.n_words = n_words;
+    a.ld = ld;
+    a.scores = scores;
+    a.temp = temp;
+    a.words = words;
+    a.logp = logp;
+    a.entropy = entropy;
+    a.top_words = top_words;
+    a.top_logp = top_logp;
+    a.part = static_cast<probs_part*>(work);
+    a.best = reinterpret_cast<word_score*>(static_cast<char*>(work) + sums);
+    return done(launch_word_probs(a, c->stream), who);
+    SH_ENTRY_END
+}
+
+int sh_tree_take(sh_ctx* c, int n, int rows, const int32_t* cu, const int32_t* parent, const int32_t* words, const int32_t* picks, const int32_t* held,
+                 const int32_t* len, int32_t* path, int32_t* count, int32_t* next, int32_t* len_out, int page, const int32_t* table, int cols,
+                 int32_t* free_pages, int n_free, const int32_t* taken, int32_t* taken_out) {
+    SH_ENTRY
+    const char* who = "sh_tree_take";
+    if (!c || n < 1 || rows < 0) return bad(who, "null context, n below 1, or rows negative");
+    if (n > PLAN_MAX_N) return bad(who, "n must be 1 to 4096");
+    if (!cu || !held || !len || !count || !next || !len_out || (rows && (!parent || !words || !picks || !path))) return bad(who, "null");
+    if (table) {
+        if (page_log(page) < 0) return bad(who, "page must be 16, 32, 64, 128 or 256");
+        if (cols < 0 || n_free < 0) return bad(who, "a size is negative");
+        if (!taken || !taken_out || (n_free && !free_pages)) return bad(who, "null");
+    }
+    const size_t each = (size_t)n * 4, row4 = (size_t)rows * 4;
+    const extent in[] = {{cu, each + 4}, {parent, row4}, {words, row4}, {picks, row4}, {held, each}, {len, each}, {table, table ? each * cols : 0},
+                         {table ? taken : nullptr, 4}},
+                 out[] = {{path, row4}, {count, each}, {next, each}, {len_out, each}, {table ? free_pages : nullptr, (size_t)(table ? n_free : 0) * 4},
+                          {table ? taken_out : nullptr, 4}};
+    if (const char* f = overlap(in, out)) return bad(who, f);
+    const on_device dev(c->device);
+    if (dev.e != hipSuccess) return done(dev.e, who);
+    tree_take_args a{};
+    a.n = n;
+    a.rows = rows;
+    a.cu = cu;
+    a.parent = parent;
+    a.word = words;
+    a.pick = picks;
+    a.held = held;
+    a.len = len;
+    a.path = path;
+    a.count = count;
+    a.next = next;
+    a.len_out = len_out;
+    if (table) {
+        a.page_log = page_log(page);
+        a.cols = cols;
+        a.n_free = n_free;
+        a.table = table;
+        a.taken = taken;
+        a.free_pages = free_pages;
+        a.taken_out = taken_out;
+    }
+    return done(launch_tree_take(a, c->stream), who);
+    SH_ENTRY_END
+}
+
+int sh_page_keep(sh_ctx* c, const sh_page_shape* s, int n, int rows, const int32_t* cu, const int32_t* path, const int32_t* len, const int32_t* table,
+                 int cols, void* keys, void* values) {
+    SH_ENTRY
+    const char* who = "sh_page_keep";
+    if (const char* f = shape_fault(s)) return bad(who, f);
+    if (!c || n < 1 || rows < 0 || cols < 0) return bad(who, "null context, n below 1, or a size is negative");
+    if (n > most_blocks(256) || (2ll * s->n_kv * (s->head_dim / 8) + 255) / 256 * n > most_blocks(256)) return bad(who, "more requests than one launch holds");
+    if (rows == 0) return SH_OK;
+    if (!cu || !path || !len || !keys || !values || (cols && !table)) return bad(who, "null");
+    if (off(keys, 16) || off(values, 16)) return bad(who, "keys and values start on 16 bytes");
+    const size_t cache = (size_t)s->n_pages * s->n_kv * s->page * s->head_dim * 2;
+    const extent in[] = {{cu, ((size_t)n + 1) * 4}, {path, (size_t)rows * 4}, {len, (size_t)n * 4}, {table, (size_t)n * cols * 4}}, out[] = {{keys, cache}, {values, cache}};
+    if (const char* f = overlap(in, out)) return bad(who, f);
+    const on_device dev(c->device);
+    if (dev.e != hipSuccess) return done(dev.e, who);
+    keep_args a{};
+    a.n = n;
+    a.rows = rows;
+    a.n_kv = s->n_kv;
+    a.page_log = page_log(s->page);
+    a.cols = cols;
+    a.n_pages = (int)s->n_pages;
+    a.cu = cu;
+    a.path = path;
+    a.len = len;
+    a.table = table;
+    a.keys = keys;
+    a.values = values;
+    return done(launch_page_keep(s->head_dim, a, c->stream), who);
     SH_ENTRY_END
 }
 
