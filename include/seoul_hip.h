@@ -434,7 +434,7 @@ int sh_tree_plan(sh_ctx* ctx, int n, int rows, const int32_t* cu, const int32_t*
 /* sh_page_attn for trees: the last cu[i + 1] - cu[i] of a request's len[i] positions are its rows' words. A row sees the shared
  * positions, its request's own before those words, and of the words those whose bits its mask has (its own bit set); its
  * position is that of the last own one before the words plus its bits, and the shape's window counts by it. A row without its
- * own bit sees nothing: zeros and -inf. Masks need not come from sh_tree_plan: any bits of the request's words are followed.
+ * own bit, or of a request whose length is less than its rows, sees nothing: zeros and -inf. Masks need not come from sh_tree_plan: any bits of the request's words are followed.
  * All else, work memory among it (sh_tree_attn_work), is as sh_page_attn says. max_rows 1 to 256; masks have
  * ceil(max_rows / 32) words a row. */
 int sh_tree_attn_work(const sh_page_shape* shape, int n, int rows, int max_rows, int prefix_len, int max_len, size_t* bytes);
@@ -450,7 +450,7 @@ int sh_tree_attn(sh_ctx* ctx, const sh_page_shape* shape, int n, int rows, const
  *   top_words, top_logp [rows][n_top]  the n_top likeliest words, by score and, among equal ones, by index, and their log
  *                              probabilities (either may be null; n_top 0 to 64)
  * temp is one value per row or null (1). temp 0 is sh_sample's greedy row: the first of the largest scores has log probability
- * 0, all others -inf; a negative or NaN temp gives NaN. Scores of -inf or NaN have log probability -inf and are not among the
+ * 0, all others -inf; a negative or NaN temp gives NaN throughout. Scores of -inf or NaN have log probability -inf and are not among the
  * likeliest (-1 and -inf where too few are left); a score of +inf shares everything with its like. Words outside [0, vocab)
  * have -inf. A row with nothing above -inf has entropy 0. vocab at most 524288. work: sh_word_probs_work's bytes, as above. */
 int sh_word_probs_work(int rows, int vocab, int n_top, size_t* bytes);

@@ -146,9 +146,9 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, joi
             const int k = SHARED ? request_of(a.cu, a.n, row[t]) : i;
             const long long first_row = a.cu[k], rows_k = a.cu[k + 1] - first_row, nth = row[t] - first_row;
             const int held = min(max(a.len[k], 0), own_max);
-            const int base = (int)max(held - rows_k, -1ll - a.rows);   // the tree's first word; negative where the request lacks some
+            const int base = (int)max(held - rows_k, 0ll);   // the tree's first word
             const unsigned* mask = a.mask + (size_t)row[t] * a.words;
-            const bool node = nth >= 0 && nth < 32ll * a.words && (mask[nth >> 5] >> (nth & 31) & 1);
+            const bool node = held >= rows_k && nth >= 0 && nth < 32ll * a.words && (mask[nth >> 5] >> (nth & 31) & 1);
             int from = 0, first_word = 0;
             if (node && a.window) {
                 int depth = -1;
@@ -174,9 +174,9 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, joi
                 hi[t] = L0;
             } else {
                 words_at = P + base;
-                lo[t] = first_word ? max(words_at + first_word, P) : from >= L0 ? P + (from - L0) : a.fused ? from : P;
+                lo[t] = first_word ? words_at + first_word : from >= L0 ? P + (from - L0) : a.fused ? from : P;
                 hi[t] = node ? P + held : lo[t];
-                sure = node ? max(words_at, P) : 0;
+                sure = node ? words_at : 0;
             }
         } else {
         if (!SHARED || a.window) {

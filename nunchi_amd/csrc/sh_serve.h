@@ -95,7 +95,6 @@ struct keep_args {
 // one part of a row of scores: its largest, how many have that value, the others' weights relative to it, and their sum times
 // the distance (in powers of two)
 struct probs_part { float top, ties, rest, dist; };
-struct word_score { float x; int i; };
 
 struct probs_args {
     int rows, vocab, type, n_words, n_top, parts, chunk;
@@ -106,7 +105,7 @@ struct probs_args {
     float *logp, *entropy, *top_logp;
     int32_t* top_words;
     probs_part* part;          // [rows][parts]
-    word_score* best;          // [rows][parts][max(n_top, 1)]
+    unsigned long long* best;  // [rows][parts][max(n_top, 1)] keys of the likeliest words, 0 where there are none
 };
 
 hipError_t launch_page_plan(const plan_args& a, hipStream_t s);

@@ -121,7 +121,7 @@ const char* probs_sizes(int rows, int vocab, int n_top, probs_args& a) {
 void probs_work(const probs_args& a, size_t* sums, size_t* all) {
     const size_t parts = (size_t)a.rows * a.parts;
     *sums = align256(parts * sizeof(probs_part));
-    *all = *sums + align256(parts * (a.n_top > 0 ? a.n_top : 1) * sizeof(word_score));
+    *all = *sums + align256(parts * (a.n_top > 0 ? a.n_top : 1) * sizeof(unsigned long long));
     if (*all < 256) *all = 256;
 }
 }  // namespace
@@ -463,7 +463,7 @@ int sh_word_probs(sh_ctx* c, int rows, int vocab, const void* scores, long long 
     a.top_words = top_words;
     a.top_logp = top_logp;
     a.part = static_cast<probs_part*>(work);
-    a.best = reinterpret_cast<word_score*>(static_cast<char*>(work) + sums);
+    a.best = reinterpret_cast<unsigned long long*>(static_cast<char*>(work) + sums);
     return done(launch_word_probs(a, c->stream), who);
     SH_ENTRY_END
 }

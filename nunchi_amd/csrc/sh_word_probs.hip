@@ -5,8 +5,10 @@
 // relative to its own largest score, of which two parts' join as in a running softmax (k_probs_join). The largest score's own
 // weight, 1, is counted apart from the others' sum (the rest): log L = log1p(rest) keeps its digits where one word has nearly
 // everything, and the entropy is a sum of two numbers that are not negative.
-// The likeliest words of a part: the n-th largest of its lanes' largest scores is no larger than its n-th largest score, so a few
-// dozen scores from there up hold them all; these are ordered by counting, for each, those before it. No histogram, no sort.
+// The likeliest words of a part: with the scores in groups, the n-th largest of the groups' largest scores is no larger than the
+// n-th largest score, so the few dozen scores from there up hold them all; these are ordered by counting, for each, those before
+// it. No histogram, no sort. A word's place in the order is one 64-bit key: its score as a number that sorts like it, and its
+// index turned round.
 #include <hip/hip_runtime.h>
 
 #include <climits>
@@ -18,7 +20,7 @@ namespace sh {
 namespace {
 
 constexpr int PT = 256;                    // threads of a part
-constexpr int LISTED = 1024;               // scores that may be listed
+constexpr int LISTED = 1024;               // words that may be listed
 
 template <class T> struct score_vec {
     static constexpr int V = 8;
@@ -29,312 +31,313 @@ template <> struct score_vec<float> {
     typedef float vec __attribute__((ext_vector_type(4), aligned(4)));
 };
 
-// scores as numbers that sort like them (-0 as 0)
+typedef unsigned long long u64;
+
+// scores as numbers that sort like them (-0 as 0); above NONE: a score that is more than -inf
 __device__ __forceinline__ unsigned order_of(float x) {
     const unsigned b = __float_as_uint(x + 0.0f);
     return b ^ ((int)b < 0 ? 0xFFFFFFFFu : 0x80000000u);
 }
-// whether word a comes before word b among the likeliest
-__device__ __forceinline__ bool ahead(float xa, int ia, float xb, int ib) { return xa > xb || (xa == xb && ia < ib); }
+constexpr unsigned NONE = 0x007FFFFFu;     // order_of(-inf)
+__device__ __forceinline__ float of_order(unsigned k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+__device__ __forceinline__ u64 key_of(float x, int i) { return (u64)order_of(x) << 32 | (unsigned)~i; }
 
-__device__ __forceinline__ int wave_sum(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+template <int CTRL, class V> __device__ __forceinline__ V by_dpp(V v) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
 }
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+template <class V> __device__ __forceinline__ V of_lane(V v, int lane) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
-__device__ __forceinline__ float wave_most(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+// the same value in every lane (the wave fully active): within each 16 lanes by DPP, then the four of them
+template <class V> __device__ __forceinline__ V wave_all(V v, V (*f)(V, V)) {
+    v = f(v, by_dpp<DPP_XOR1>(v));
+    v = f(v, by_dpp<DPP_XOR2>(v));
+    v = f(v, by_dpp<DPP_MIRROR8>(v));
+    v = f(v, by_dpp<DPP_MIRROR16>(v));
+    return f(f(of_lane(v, 0), of_lane(v, 16)), f(of_lane(v, 32), of_lane(v, 48)));
 }
+__device__ __forceinline__ int add_i(int x, int y) { return x + y; }
+__device__ __forceinline__ float add_f(float x, float y) { return x + y; }
+__device__ __forceinline__ float most_f(float x, float y) { return fmaxf(x, y); }
+__device__ __forceinline__ unsigned most_u(unsigned x, unsigned y) { return max(x, y); }
 
-// the n-th largest of a wave's 64 keys (1 <= n <= 64), bit by bit
-__device__ __forceinline__ unsigned nth_of_wave(unsigned key, int n) {
-    unsigned at = 0;
+// A number that at least n of the wave's keys (N a lane) reach, and at most a few more than n: the n-th largest bit by bit, until
+// that is so.
+template <class K, int N> __device__ __forceinline__ K reached_by(const K (&key)[N], int n) {
+    K at = 0;
 #pragma unroll 1
-    for (unsigned bit = 0x80000000u; bit; bit >>= 1) {
-        const int c = __popcll(__ballot(key >= (at | bit)));
+    for (K bit = (K)1 << (8 * sizeof(K) - 1); bit; bit >>= 1) {
+        int c = 0;
+#pragma unroll
+        for (int e = 0; e < N; e++) c += __popcll(__ballot(key[e] >= (at | bit)));
         if (c >= n) at |= bit;
-        if (c == n) break;                 // (the keys from here up are the ones)
+        if (c >= n && c <= n + 4) break;
     }
     return at;
 }
 
-struct part_shared {
-    float x[LISTED];
-    int i[LISTED];
-    unsigned cut[PT / 64];
-    probs_part part[PT / 64];
-    int n, equal[PT / 64];
-};
-
-// the parts' sums as one, relative to the largest (each lane the same parts)
-__device__ __forceinline__ probs_part joined(const probs_part& a, const probs_part& b, float c) {
-    const bool first = a.top >= b.top;
-    const probs_part &hi = first ? a : b, &lo = first ? b : a;
-    probs_part r = hi;
-    if (lo.top == -INFINITY) return r;
-    if (lo.top == hi.top) {
-        r.ties += lo.ties;
-        r.rest += lo.rest;
-        r.dist += lo.dist;
-        return r;
+// The want largest of n keys in LDS, in order, to best[0 .. want); 0 behind them. One wave.
+__device__ __forceinline__ void order_keys(const u64* key, int n, int want, u64* best, int lane) {
+    if (n <= 64) {                         // one a lane, told to all lanes one after the other
+        const u64 mine = lane < n ? key[lane] : 0;
+        const int hi = (int)(mine >> 32), lo = (int)(unsigned)mine;
+        int before = 0;
+        for (int o = 0; o < n; o++) {
+            const u64 x = (u64)(unsigned)__builtin_amdgcn_readlane(hi, o) << 32 | (unsigned)__builtin_amdgcn_readlane(lo, o);
+            before += x > mine;
+        }
+        if (lane < n && before < want) best[before] = mine;
+    } else {
+        for (int k = lane; k < n; k += 64) {
+            const u64 mine = key[k];
+            int before = 0;
+#pragma unroll 8
+            for (int o = 0; o < n; o++) before += key[o] > mine;
+            if (before < want) best[before] = mine;
+        }
     }
-    if (hi.top == INFINITY) return r;
-    const float d = fmaxf((lo.top - hi.top) * c, -1000.0f), f = __builtin_amdgcn_exp2f(d), all = lo.ties + lo.rest;
-    r.rest += all * f;
-    r.dist += (lo.dist + all * d) * f;
+    for (int k = n + lane; k < want; k += 64) best[k] = 0;
+}
+
+// two parts' sums as one, relative to the larger of their largest (c: powers of two a unit of score)
+__device__ __forceinline__ probs_part joined(const probs_part& a, const probs_part& b, float c) {
+    const float top = fmaxf(a.top, b.top);
+    probs_part r{top, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const probs_part& q = k ? b : a;
+        if (q.top == top) {
+            r.ties += q.ties;
+            r.rest += q.rest;
+            r.dist += q.dist;
+        } else if (q.top > -INFINITY && top < INFINITY) {
+            const float d = fmaxf((q.top - top) * c, -200.0f), f = __builtin_amdgcn_exp2f(d), all = q.ties + q.rest;
+            r.rest += all * f;
+            r.dist += (q.dist + all * d) * f;
+        }
+    }
     return r;
 }
 
-// A part: `chunk` words of a row. VPT: words a thread
-template <class T, int VPT> __global__ __launch_bounds__(PT) void k_probs_part(probs_args a) {
-    typedef score_vec<T> sv;
-    constexpr int V = sv::V, N = VPT / V;
-    __shared__ part_shared s;
+// log2 e over the temperature, inside the range so that 0 times it is 0 (a row without a temperature above 0 has no sums)
+__device__ __forceinline__ float per_score(float temp) { return temp > 0.0f ? fminf(1.44269504f / temp, 3e38f) : 1.0f; }
+
+struct join_shared {
+    u64 key[LISTED], best[PROBS_MAX_TOP];
+    float log_sum, top;
+};
+
+// A row's parts joined, by NT threads: one wave puts the likeliest words in order, another adds up the sums.
+template <class T, int NT> __device__ __forceinline__ void join_row(const probs_args& a, const int row, join_shared& s) {
     const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
-    const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
-    const int first = part * a.chunk;
-    const T* src = (const T*)a.scores + (size_t)row * a.ld;
-    const float temp = a.temp ? a.temp[row] : 1.0f;
-    // ---- the part's scores: words that are none (NaN, past the row) are -inf ----
-    float x[VPT];
-#pragma unroll
-    for (int l = 0; l < N; l++) {
-        const int at = first + (l * PT + t) * V;
-        if (at + V <= a.vocab) {
-            const typename sv::vec v = *(const typename sv::vec*)(src + at);
-#pragma unroll
-            for (int e = 0; e < V; e++) x[l * V + e] = fmaxf((float)v[e], -INFINITY);
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; e++) x[l * V + e] = at + e < a.vocab ? fmaxf((float)src[at + e], -INFINITY) : -INFINITY;
-        }
-    }
-    float mine = x[0];
-#pragma unroll
-    for (int e = 1; e < VPT; e++) mine = fmaxf(mine, x[e]);
-    const float top = wave_most(mine);
-    // ---- sums of the wave relative to its largest ----
-    // (log2 e over the temperature, held inside the range so that 0 times it is 0; a row without one has no sums)
-    const float c = temp > 0.0f ? fminf(1.44269504f / temp, 3e38f) : 1.0f;
-    float rest[4] = {0, 0, 0, 0}, dist[4] = {0, 0, 0, 0};
-    int ties = 0;
-    const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-    for (int e = 0; e < VPT; e++) {
-        const bool same = x[e] == ref;
-        ties += __popcll(__ballot(same));
-        // (at -200 a weight is 0; scores at the largest are counted, not summed. +inf less +inf is NaN, which the maximum drops)
-        const float z = same ? -200.0f : fmaxf((x[e] - ref) * c, -200.0f);
-        const float w = __builtin_amdgcn_exp2f(z);
-        rest[e & 3] += w;
-        dist[e & 3] = fmaf(w, z, dist[e & 3]);
-    }
-    const float rest_w = wave_sum((rest[0] + rest[1]) + (rest[2] + rest[3])), dist_w = wave_sum((dist[0] + dist[1]) + (dist[2] + dist[3]));
-    if (lane == 0) s.part[wv] = probs_part{top, top == -INFINITY ? 0.0f : (float)ties, rest_w, dist_w};
-    // ---- where the likeliest begin ----
-    const int want = a.n_top > 0 ? a.n_top : 1;
-    const unsigned none = order_of(-INFINITY);
-    const unsigned cut_w = nth_of_wave(order_of(mine), want);
-    if (lane == 0) s.cut[wv] = cut_w;
-    if (t == 0) s.n = 0;
-    __syncthreads();
-    if (t == 0) {
-        probs_part p = s.part[0];
-        for (int w = 1; w < PT / 64; w++) p = joined(p, s.part[w], c);
-        a.part[(size_t)row * a.parts + part] = p;
-    }
-    unsigned cut = none + 1;
-#pragma unroll
-    for (int w = 0; w < PT / 64; w++) cut = max(cut, s.cut[w]);
-    auto index = [&](int e) { return first + ((e / V) * PT + t) * V + e % V; };
-    if (order_of(mine) >= cut) {
-#pragma unroll
-        for (int e = 0; e < VPT; e++)
-            if (order_of(x[e]) >= cut) {
-                const int at = atomicAdd(&s.n, 1);
-                if (at < LISTED) {
-                    s.x[at] = x[e];
-                    s.i[at] = index(e);
-                }
-            }
-    }
-    __syncthreads();
-    int n = s.n;
-    if (n > LISTED) {
-        // Rare (many equal scores, or many words of few lanes): the score of the last word that counts, bit by bit over all
-        // words, then the index behind the last of those equal to it
-        auto total = [&](auto&& test) {
-            int k = 0;
-#pragma unroll
-            for (int e = 0; e < VPT; e++) k += __popcll(__ballot(test(e)));
-            __syncthreads();
-            if (lane == 0) s.equal[wv] = k;
-            __syncthreads();
-            int all = 0;
-            for (int w = 0; w < PT / 64; w++) all += s.equal[w];
-            return all;
-        };
-        unsigned at = 0;
-#pragma unroll 1
-        for (unsigned bit = 0x80000000u; bit; bit >>= 1)
-            if (total([&](int e) { return order_of(x[e]) >= (at | bit); }) >= want) at |= bit;
-        const int above = total([&](int e) { return order_of(x[e]) > at; });
-        int behind = 0;                    // of the equal ones those before this index count
-#pragma unroll 1
-        for (int bit = 1 << 30; bit; bit >>= 1)
-            if (total([&](int e) { return order_of(x[e]) == at && index(e) < (behind | bit); }) <= want - above) behind |= bit;
-        if (t == 0) s.n = 0;
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < VPT; e++)
-            if (order_of(x[e]) > at || (order_of(x[e]) == at && index(e) < behind)) {
-                const int to = atomicAdd(&s.n, 1);
-                if (to < LISTED) {
-                    s.x[to] = x[e];
-                    s.i[to] = index(e);
-                }
-            }
-        __syncthreads();
-        n = min(s.n, LISTED);
-    }
-    // ---- in their order ----
-    word_score* best = a.best + ((size_t)row * a.parts + part) * want;
-    for (int k = t; k < n; k += PT) {
-        const float xk = s.x[k];
-        const int ik = s.i[k];
-        int before = 0;
-        for (int o = 0; o < n; o++) before += ahead(s.x[o], s.i[o], xk, ik);
-        if (before < want) best[before] = word_score{xk, ik};
-    }
-    for (int k = n + t; k < want; k += PT) best[k] = word_score{-INFINITY, -1};
-}
-
-constexpr int JOIN_T = 256;
-
-// A row's parts joined, its words' log probabilities
-template <class T> __global__ __launch_bounds__(JOIN_T) void k_probs_join(probs_args a) {
-    __shared__ float x_s[LISTED];
-    __shared__ int i_s[LISTED];
-    __shared__ int n_s;
-    __shared__ unsigned cut_s[JOIN_T / 64];
-    __shared__ word_score best_s[PROBS_MAX_TOP];
-    __shared__ double log_s;
-    __shared__ float top_s;
-    const int row = blockIdx.x, t = threadIdx.x, lane = t & 63, wv = t >> 6;
     const float temp = a.temp ? a.temp[row] : 1.0f;
     const int want = a.n_top > 0 ? a.n_top : 1;
-    // ---- the sums, by the first wave, in 64 bits ----
     if (wv == 0) {
-        const probs_part* p = a.part + (size_t)row * a.parts;
-        float top = -INFINITY;
-        for (int k = lane; k < a.parts; k += 64) top = fmaxf(top, p[k].top);
-        top = wave_most(top);
-        double ties = 0.0, rest = 0.0, dist = 0.0;
-        if (top > -INFINITY && temp > 0.0f) {
-            const float c = fminf(1.44269504f / temp, 3e38f);
-            for (int k = lane; k < a.parts; k += 64) {
-                const probs_part q = p[k];
-                if (q.top == top) {
-                    ties += q.ties;
-                    if (top < INFINITY) {
-                        rest += q.rest;
-                        dist += q.dist;
-                    }
-                } else if (q.top > -INFINITY && top < INFINITY) {
-                    const double d = fmax((double)(q.top - top) * c, -1000.0), f = exp2(d), all = (double)q.ties + q.rest;
-                    rest += all * f;
-                    dist += (q.dist + all * d) * f;
-                }
+        // The want-th largest of the lanes' largest keys: the few from there up hold them all
+        const u64* best = a.best + (size_t)row * a.parts * want;
+        const int all = a.parts * want;
+        u64 most = 0;
+#pragma unroll 4
+        for (int k = lane; k < all; k += 64) most = max(most, best[k]);
+        const u64 mosts[1] = {most}, cut = max(reached_by(mosts, want), 1ull);
+        int n = 0;
+#pragma unroll 4
+        for (int k = 0; k < all; k += 64) {
+            const u64 mine = k + lane < all ? best[k + lane] : 0;
+            const u64 who = __ballot(mine >= cut);
+            const int at = n + __popcll(who & ((1ull << lane) - 1));
+            if (mine >= cut && at < LISTED) s.key[at] = mine;
+            n += __popcll(who);
+        }
+        if (n <= LISTED) {
+            order_keys(s.key, n, want, s.best, lane);
+        } else {                           // (hundreds of parts of which a few lanes hold most of the likeliest)
+            for (int k = lane; k < all; k += 64) {
+                const u64 mine = best[k];
+                if (mine < cut) continue;
+                int before = 0;
+                for (int o = 0; o < all && before < want; o++) before += best[o] > mine;
+                if (before < want) s.best[before] = mine;
             }
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            ties += __shfl_xor(ties, o);
-            rest += __shfl_xor(rest, o);
-            dist += __shfl_xor(dist, o);
+    } else if (wv == 1) {
+        const probs_part* p = a.part + (size_t)row * a.parts;
+        const float c = per_score(temp);
+        probs_part q{-INFINITY, 0.0f, 0.0f, 0.0f};
+        for (int k = lane; k < a.parts; k += 64) q = joined(q, p[k], c);
+        const float top = wave_all(q.top, most_f);
+        if (q.top < top) {
+            const probs_part at_top{top, 0.0f, 0.0f, 0.0f};
+            q = joined(q, at_top, c);
         }
+        const float ties = wave_all(q.ties, add_f), rest = wave_all(q.rest, add_f), dist = wave_all(q.dist, add_f);
         if (lane == 0) {
-            const double log_sum = ties > 1.0 ? log(ties + rest) : log1p(rest);
-            log_s = log_sum;
-            top_s = top;
+            const float log_sum = ties > 1.0f ? logf(ties + rest) : log1pf(rest);
+            s.log_sum = log_sum;
+            s.top = top;
             if (a.entropy) {
                 float h = 0.0f;
-                if (temp > 0.0f && top > -INFINITY) h = (float)(log_sum - dist * 0.6931471805599453 / (ties + rest));
+                if (temp > 0.0f && top > -INFINITY) h = log_sum - dist * 0.69314718f / (ties + rest);
                 else if (!(temp >= 0.0f)) h = NAN;
                 a.entropy[row] = h;
             }
         }
     }
-    // ---- the likeliest words of all parts: from the largest of the parts' last ones up ----
-    const word_score* best = a.best + (size_t)row * a.parts * want;
-    unsigned cut = order_of(-INFINITY) + 1;
-    for (int k = t; k < a.parts; k += JOIN_T) cut = max(cut, order_of(best[(size_t)k * want + want - 1].x));
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) cut = max(cut, (unsigned)__shfl_xor((int)cut, o));
-    if (lane == 0) cut_s[wv] = cut;
-    if (t == 0) n_s = 0;
-    if (t < want) best_s[t] = word_score{-INFINITY, -1};
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < JOIN_T / 64; w++) cut = max(cut, cut_s[w]);
-    for (int k = t; k < a.parts * want; k += JOIN_T) {
-        const word_score b = best[k];
-        if (order_of(b.x) >= cut) {
-            const int at = atomicAdd(&n_s, 1);
-            if (at < LISTED) {
-                x_s[at] = b.x;
-                i_s[at] = b.i;
-            }
-        }
-    }
-    __syncthreads();
-    const int listed = n_s;
-    if (listed <= LISTED) {
-        for (int k = t; k < listed; k += JOIN_T) {
-            const float xk = x_s[k];
-            const int ik = i_s[k];
-            int before = 0;
-            for (int o = 0; o < listed; o++) before += ahead(x_s[o], i_s[o], xk, ik);
-            if (before < want) best_s[before] = word_score{xk, ik};
-        }
-    } else {
-        // (many parts whose words are equal)
-        for (int k = t; k < a.parts * want; k += JOIN_T) {
-            const word_score b = best[k];
-            if (order_of(b.x) < cut) continue;
-            int before = 0;
-            for (int o = 0; o < a.parts * want && before < want; o++) before += best[o].i >= 0 && ahead(best[o].x, best[o].i, b.x, b.i);
-            if (before < want) best_s[before] = b;
-        }
-    }
-    __syncthreads();
-    const float top = top_s;
-    const int first = best_s[0].i;
+    const float top = s.top, log_sum = s.log_sum;
+    const int first = (int)~(unsigned)s.best[0];
     auto logp = [&](float x, int i) {
         if (!(temp >= 0.0f)) return (float)NAN;
         if (!(x > -INFINITY)) return -INFINITY;
         if (temp == 0.0f) return i == first ? 0.0f : -INFINITY;
-        if (top == INFINITY && x < top) return -INFINITY;
-        const double z = x == top ? 0.0 : ((double)x - top) / temp;
-        return (float)(z - log_s);
+        if (x == top) return -log_sum;
+        if (top == INFINITY) return -INFINITY;
+        return (x - top) / temp - log_sum;
     };
-    for (int k = t; k < a.n_top; k += JOIN_T) {
-        const word_score b = best_s[k];
-        if (a.top_words) a.top_words[(size_t)row * a.n_top + k] = b.i;
-        if (a.top_logp) a.top_logp[(size_t)row * a.n_top + k] = logp(b.x, b.i);
+    for (int k = t; k < a.n_top; k += NT) {
+        const u64 b = s.best[k];
+        const size_t at = (size_t)row * a.n_top + k;
+        if (a.top_words) a.top_words[at] = b ? (int)~(unsigned)b : -1;
+        if (a.top_logp) a.top_logp[at] = b ? logp(of_order((unsigned)(b >> 32)), (int)~(unsigned)b) : temp >= 0.0f ? -INFINITY : (float)NAN;
     }
-    for (int k = t; k < a.n_words; k += JOIN_T) {
+    for (int k = t; k < a.n_words; k += NT) {
         const int w = a.words[(size_t)row * a.n_words + k];
         const float x = w >= 0 && w < a.vocab ? (float)((const T*)a.scores)[(size_t)row * a.ld + w] : -INFINITY;
         a.logp[(size_t)row * a.n_words + k] = logp(x, w);
     }
+}
+
+// A part: PT * VPT words of a row, VPT a thread. A row that is one part is finished here.
+template <class T, int VPT> __global__ __launch_bounds__(PT) void k_probs_part(probs_args a) {
+    typedef score_vec<T> sv;
+    constexpr int V = sv::V, N = VPT / V, WAVES = PT / 64;
+    __shared__ join_shared js;
+    u64* const key_s = js.key;
+    __shared__ unsigned lane_s[PT], cut_s;
+    __shared__ probs_part part_s[WAVES];
+    __shared__ int n_s, count_s[WAVES];
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+    const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+    const int first = part * (PT * VPT);
+    const T* src = (const T*)a.scores + (size_t)row * a.ld;
+    const float c = per_score(a.temp ? a.temp[row] : 1.0f);
+    // ---- the part's scores, behind the row's end -inf: all loads before the first is waited for ----
+    // (a vector that would pass the end is taken from the row's last words, of which those before its place do not count)
+    auto place = [&](int l) { return first + (l * PT + t) * V; };
+    auto from = [&](int l) { return max(min(place(l), a.vocab - V), 0); };
+    float x[VPT];
+    if (a.vocab >= V) {
+        typename sv::vec v[N];
+#pragma unroll
+        for (int l = 0; l < N; l++) v[l] = *(const typename sv::vec*)(src + from(l));
+#pragma unroll
+        for (int l = 0; l < N; l++)
+#pragma unroll
+            for (int e = 0; e < V; e++) x[l * V + e] = (float)v[l][e];
+    } else {
+#pragma unroll
+        for (int l = 0; l < N; l++)
+#pragma unroll
+            for (int e = 0; e < V; e++) x[l * V + e] = (float)src[min(e, a.vocab - 1)];
+    }
+    if (first + PT * VPT > a.vocab) {
+#pragma unroll
+        for (int l = 0; l < N; l++)
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                if (from(l) + e < place(l) || from(l) + e >= a.vocab) x[l * V + e] = -INFINITY;
+    }
+    float mine = -INFINITY;                // (NaN is passed over here and in every comparison below)
+#pragma unroll
+    for (int e = 0; e < VPT; e++) mine = fmaxf(mine, x[e]);
+    lane_s[t] = order_of(mine);
+    const float top = wave_all(mine, most_f);
+    // ---- sums of the wave relative to its largest ----
+    float rest[2] = {0, 0}, dist[2] = {0, 0};
+    int ties = 0;
+    const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int e = 0; e < VPT; e++) {
+        const bool same = x[e] == ref;
+        ties += same;
+        // (at -200 a weight is 0; scores at the largest are counted, not summed. +inf less +inf is NaN, which the maximum drops)
+        const float z = same ? -200.0f : fmaxf((x[e] - ref) * c, -200.0f);
+        const float w = __builtin_amdgcn_exp2f(z);
+        rest[e & 1] += w;
+        dist[e & 1] = fmaf(w, z, dist[e & 1]);
+    }
+    ties = wave_all(ties, add_i);
+    const float rest_w = wave_all(rest[0] + rest[1], add_f), dist_w = wave_all(dist[0] + dist[1], add_f);
+    if (lane == 0) part_s[wv] = probs_part{top, top == -INFINITY ? 0.0f : (float)ties, rest_w, dist_w};
+    if (t == 0) n_s = 0;
+    __syncthreads();
+    // ---- where the likeliest begin: groups of four threads' words, or of one's where more than 32 are asked for ----
+    const int want = a.n_top > 0 ? a.n_top : 1;
+    if (wv == 0) {
+        unsigned k[4];
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) k[w] = lane_s[64 * w + lane];
+        unsigned cut;
+        if (want <= 32) {
+            const unsigned all[1] = {max(max(k[0], k[1]), max(k[2], k[3]))};
+            cut = reached_by(all, want);
+        } else {
+            cut = reached_by(k, want);
+        }
+        if (lane == 0) cut_s = max(cut, NONE + 1);
+    } else if (t == 64) {
+        probs_part p = part_s[0];
+        for (int w = 1; w < WAVES; w++) p = joined(p, part_s[w], c);
+        a.part[(size_t)row * a.parts + part] = p;
+    }
+    __syncthreads();
+    const float cut = of_order(cut_s);
+    auto index = [&](int e) { return from(e / V) + e % V; };
+    if (mine >= cut) {
+#pragma unroll
+        for (int e = 0; e < VPT; e++)
+            if (x[e] >= cut) {
+                const int at = atomicAdd(&n_s, 1);
+                if (at < LISTED) key_s[at] = key_of(x[e], index(e));
+            }
+    }
+    __syncthreads();
+    int n = n_s;
+    if (n > LISTED) {
+        // Rare (many equal scores, or most of the likeliest with few threads): the key of the last word that counts, bit by bit
+        // over all words
+        u64 at = 0;
+#pragma unroll 1
+        for (u64 bit = 1ull << 63; bit; bit >>= 1) {
+            int k = 0;
+#pragma unroll
+            for (int e = 0; e < VPT; e++) k += x[e] >= cut && key_of(x[e], index(e)) >= (at | bit);
+            k = wave_all(k, add_i);
+            __syncthreads();
+            if (lane == 0) count_s[wv] = k;
+            __syncthreads();
+            if (count_s[0] + count_s[1] + count_s[2] + count_s[3] >= want) at |= bit;
+        }
+        if (t == 0) n_s = 0;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < VPT; e++)
+            if (x[e] >= cut && key_of(x[e], index(e)) >= at) key_s[atomicAdd(&n_s, 1) & (LISTED - 1)] = key_of(x[e], index(e));
+        __syncthreads();
+        n = min(n_s, LISTED);
+    }
+    if (wv == 0) order_keys(key_s, n, want, a.best + ((size_t)row * a.parts + part) * want, lane);
+    if (a.parts == 1) {
+        __syncthreads();
+        join_row<T, PT>(a, row, js);
+    }
+}
+
+constexpr int JOIN_T = 128;
+
+template <class T> __global__ __launch_bounds__(JOIN_T) void k_probs_join(probs_args a) {
+    __shared__ join_shared s;
+    join_row<T, JOIN_T>(a, blockIdx.x, s);
 }
 
 template <class T> hipError_t run_probs(const probs_args& a, hipStream_t s) {
@@ -343,15 +346,17 @@ template <class T> hipError_t run_probs(const probs_args& a, hipStream_t s) {
     else k_probs_part<T, 32><<<grid, PT, 0, s>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    k_probs_join<T><<<dim3((unsigned)a.rows), JOIN_T, 0, s>>>(a);
+    if (a.parts > 1) k_probs_join<T><<<dim3((unsigned)a.rows), JOIN_T, 0, s>>>(a);
     return hipGetLastError();
 }
 
 }  // namespace
 
-// Parts of 8192 words, or of 2048 where the rows are too few to fill the compute units with those.
+// One part where 8192 words hold the row, so that one launch is all. Else parts of 8192 words, or of 2048 where the rows are too
+// few to fill the compute units with those.
 void word_probs_split(probs_args& a) {
-    a.chunk = (long long)a.rows * ((a.vocab + 8191) / 8192) >= 512 ? 8192 : 2048;
+    const int large = 32 * PT, small = 8 * PT;
+    a.chunk = a.vocab <= small ? small : a.vocab <= large || (long long)a.rows * ((a.vocab + large - 1) / large) >= 512 ? large : small;
     a.parts = (a.vocab + a.chunk - 1) / a.chunk;
 }
 
