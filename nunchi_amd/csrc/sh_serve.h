@@ -115,6 +115,7 @@ hipError_t launch_page_put(int D, int src_type, int type, const put_args& a, hip
 bool page_attn_split(int D, bool single, pattn_args& a);
 hipError_t launch_page_attn(int D, int type, const pattn_args& a, hipStream_t s);
 // the same with trees of drafted words (a.mask)
+bool tree_attn_split(int D, pattn_args& a);
 hipError_t launch_tree_attn(int D, int type, const pattn_args& a, hipStream_t s);
 // the parts of a call joined; nothing where there is one
 hipError_t launch_page_join(int D, int type, const pattn_args& a, hipStream_t s);

@@ -75,7 +75,7 @@ const char* shape_fault(const sh_page_shape* s) {
 }
 
 // sizes of an attention call into its argument block (the parts of the keys among them); null when they are in range
-const char* attn_sizes(const sh_page_shape* s, int n, int rows, int max_rows, int prefix_len, int max_len, bool single, pattn_args& a) {
+const char* attn_sizes(const sh_page_shape* s, int n, int rows, int max_rows, int prefix_len, int max_len, bool single, pattn_args& a, bool tree = false) {
     if (const char* f = shape_fault(s)) return f;
     if (n < 1 || rows < 0 || max_rows < 1 || prefix_len < 0 || max_len < 0) return "a size is negative, or n or max_rows is 0";
     if (single && (rows != n || max_rows != 1)) return "without cu every request has one row (rows == n, max_rows == 1)";
@@ -92,7 +92,7 @@ const char* attn_sizes(const sh_page_shape* s, int n, int rows, int max_rows, in
     a.max_len = max_len;
     a.n_pages = (int)s->n_pages;
     a.c = std::fmax((s->scale > 0.0f ? s->scale : 1.0f / std::sqrt((float)s->head_dim)) * 1.44269504f, FLT_MIN);   // (0 times a masked -inf is NaN)
-    if (!page_attn_split(s->head_dim, single, a)) return "more workgroups than one launch holds: fewer rows at once";
+    if (!(tree ? tree_attn_split(s->head_dim, a) : page_attn_split(s->head_dim, single, a))) return "more workgroups than one launch holds: fewer rows at once";
     return nullptr;
 }
 
@@ -366,7 +366,7 @@ int sh_tree_attn_work(const sh_page_shape* s, int n, int rows, int max_rows, int
     *bytes = 0;
     if (max_rows > TREE_MAX) return bad(who, "max_rows must be 1 to 256");
     pattn_args a{};
-    if (const char* f = attn_sizes(s, n, rows, max_rows, prefix_len, max_len, false, a)) return bad(who, f);
+    if (const char* f = attn_sizes(s, n, rows, max_rows, prefix_len, max_len, false, a, true)) return bad(who, f);
     size_t sums;
     attn_work(a, s->head_dim, &sums, bytes);
     if (*bytes < 256) *bytes = 256;
@@ -381,7 +381,7 @@ int sh_tree_attn(sh_ctx* c, const sh_page_shape* s, int n, int rows, const int32
     const char* who = "sh_tree_attn";
     if (max_rows > TREE_MAX) return bad(who, "max_rows must be 1 to 256");
     pattn_args a{};
-    if (const char* f = attn_sizes(s, n, rows, max_rows, prefix_len, max_len, false, a)) return bad(who, f);
+    if (const char* f = attn_sizes(s, n, rows, max_rows, prefix_len, max_len, false, a, true)) return bad(who, f);
     if (!c) return bad(who, "null context");
     if (rows == 0) return SH_OK;
     if (!cu || !mask || !q || !keys || !values || !len || !out || (prefix_len && !prefix) || cols < 0 || (cols && !table)) return bad(who, "null, or cols negative");

@@ -1,30 +1,572 @@
-// Attention of a batch whose requests try a tree of drafted words each (sh_tree_attn): the workgroups of sh_attend.h, in which
-// a row sees of its request's last positions those whose bits its mask has. The parts are joined by sh_page_attn.hip's kernel.
+// Attention of a batch whose requests try a tree of drafted words each (sh_tree_attn): every word sees the shared positions, its
+// request's own before the tree and the words that it follows. Parts of the keys are taken by workgroups of their own and
+// joined after them by sh_page_attn.hip's kernel.
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
 
 #include "sh_attend.h"
 
 namespace sh {
 namespace {
 
+constexpr int MASK_WORDS = TREE_MAX / 32;
+
+template <int D, int NT> struct tree_space {
+    union {
+        join_space<D, NT> join;
+        unsigned short keys[4][32 * (D + 8)];  // each wave's block of keys (the pitch shifts rows by four banks)
+    };
+    unsigned mask[16 * NT][MASK_WORDS + 1];    // the columns' masks, and a word without bits
+    int lo[16 * NT], hi[16 * NT];              // what a column sees (below)
+    float top[4][16 * NT];                     // the largest score of each wave's first block
+};
+
+// four bits from bit `from` on of a column's mask; what lies before the first word is set
+__device__ __forceinline__ unsigned tree_bits(const unsigned* mask, int words, int from) {
+    if (from <= -4) return 0xFu;
+    if (from < 0) return ((mask[0] << -from) | ((1u << -from) - 1)) & 0xFu;
+    const int w = min(from >> 5, words);
+    const unsigned long long two = mask[w] | (unsigned long long)mask[min(w + 1, words)] << 32;
+    return (unsigned)(two >> (from & 31)) & 0xFu;
+}
+
+// the largest of four lanes 16 apart
+__device__ __forceinline__ float over_quads(float x) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// The last request k with f(cu[k], k) <= at (f(cu[0], 0) <= at, f does not fall), its row starts and its length: a wave looks at
+// 64 requests at a time.
+struct found_request {
+    int k, cu0, cu1, len;
+};
+template <class F> __device__ __forceinline__ found_request find_request(const pattn_args& a, int at, int lane, F f) {
+    int lo = 0, hi = a.n;
+    for (;;) {
+        const int step = (hi - lo + 62) / 63, k = lo + lane * step;
+        const int cu = a.cu[min(k, a.n)], len = a.len[min(k, a.n - 1)];
+        const int there = max(__popcll(__ballot(k < hi && f(cu, k) <= at)), 1);
+        lo += (there - 1) * step;
+        if (step == 1)
+            return {lo, __builtin_amdgcn_readlane(cu, there - 1), __builtin_amdgcn_readlane(cu, there), __builtin_amdgcn_readlane(len, there - 1)};
+        hi = min(hi, lo + step);
+    }
+}
+
+// Keys are counted along one line: the shared positions, a gap to the next multiple of 32, the request's own, of which the last
+// are its tree's words. Columns: the (row, query head) pairs of one kv head, packed; a workgroup takes 16 NT of them and one part
+// of the line, its four waves take blocks of 32 keys in turn. With K of 32 keys as rows of the first product (S^T = K Q^T) a
+// lane holds the scores of one column, so maxima and sums stay in the lane: four of either half of the block's keys, which are its
+// operand of the second product (O^T = V^T P^T) as they are, if V's rows are dealt the same way. V's operand is eight keys of one
+// dimension: each lane loads the same D / 16 dimensions of its eight keys and turns the block with byte permutes. A load takes
+// rows of one half, so its address is the wave's and a lane's place in it never changes. Keys are asked for as soon as the first
+// product has read those before them, values as soon as the second has: loads are in flight all the time without registers of
+// their own.
+// Weights are rounded to the values' 16 bits for the second product; their sum stays in 32 bits. They are relative to a maximum
+// that is up to 2^SLACK behind the true one and 2^LIFT below it (sh_page_attn.hip says why). Each column is rescaled by its own
+// scores alone, so a row's result does not depend on the rows beside it.
+// SHARED: the columns of all requests over the shared positions. Else one request's columns over its own positions, and over the
+// shared ones before them where no SHARED part takes them (a.fused).
+template <class T, int D, int NT, bool SHARED>
+__device__ __forceinline__ void attend(const pattn_args& a, const int block, tree_space<D, NT>& s) {
+    constexpr int NC = 16 * NT, E = D / 16, CH = D / 32, VW = E / 2, PITCH = join_space<D, NT>::PITCH;
+    // f16 weights up to 2^15: their last place is 2^-32 of the largest or less, which a million keys add up to a quarter of half a place
+    constexpr float LIFT = mat<T>::LIFT > 0.0f ? 8.0f : 0.0f, SLACK = mat<T>::LIFT > 0.0f ? 7.0f : mat<T>::SLACK;
+    join_space<D, NT>& js = s.join;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m16 = lane & 15, quad = lane >> 4;
+    const int S = SHARED ? a.sp : a.so, per = a.n_kv * S;
+    // (workgroups of the same keys are `per` apart: on one XCD where that is a multiple of 8)
+    const int gs = block % per, g = gs % a.n_kv, part = gs / a.n_kv;
+    const int tile = block / per;
+    // ---- the workgroup's columns ----
+    int i = 0, r0 = 0, r1, ct = tile;      // request, its rows, tile of columns within them
+    [[maybe_unused]] found_request mine{};
+    if constexpr (SHARED) {
+        r1 = min(max(a.cu[a.n], 0), a.rows);
+    } else {
+        // request i owns the tiles first(i) .. first(i + 1) - 1, at least as many as its columns fill
+        auto row_at = [&](int cu) { return min(max(cu, 0), a.rows); };
+        auto first = [&](int cu, int k) { return (int)((long long)row_at(cu) * a.grp / NC) + k; };
+        mine = find_request(a, tile, lane, first);
+        i = mine.k;
+        ct = tile - first(mine.cu0, i);
+        r0 = row_at(mine.cu0);
+        r1 = min(row_at(mine.cu1), r0 + a.max_rows);
+    }
+    const int ncol = (r1 - r0) * a.grp, c0 = ct * NC;
+    if (c0 < 0 || c0 >= ncol) return;
+    auto row_of = [&](int c) { return r0 + min(c0 + c, ncol - 1) / a.grp; };
+    auto head_of = [&](int c) { return g * a.grp + min(c0 + c, ncol - 1) % a.grp; };
+    for (int k = threadIdx.x; k < NC * (a.words + 1); k += 256) {
+        const int c = k / (a.words + 1), w = k - c * (a.words + 1);
+        s.mask[c][w] = w < a.words ? a.mask[(size_t)row_of(c) * a.words + w] : 0u;
+    }
+    u32x4 qf[CH][NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int c = 0; c < CH; c++)
+            qf[c][t] = *(const u32x4*)((const T*)a.q + ((size_t)row_of(16 * t + m16) * a.n_head + head_of(16 * t + m16)) * D + c * 32 + quad * 8);
+    __syncthreads();
+    // ---- what each column sees: of keys lo .. hi - 1 all before words_at, and the words there whose bits its mask has ----
+    const int L0 = a.prefix_len, P = a.own_at;
+    const int own_max = (int)min((long long)a.max_len, (long long)a.cols << a.page_log);
+    int words_at = L0;
+    int lo0 = INT_MAX, lo1 = 0, hi0 = INT_MAX, hi1 = 0;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const int c = 16 * t + m16, row = row_of(c);
+        const unsigned* mask = s.mask[c];
+        const int k = SHARED ? request_of(a.cu, a.n, row) : i;
+        const long long first_row = SHARED ? a.cu[k] : mine.cu0, rows_k = (SHARED ? a.cu[k + 1] : mine.cu1) - first_row, nth = row - first_row;
+        const int held = min(max(SHARED ? a.len[k] : mine.len, 0), own_max);
+        const int base = (int)max(held - rows_k, 0ll);   // the tree's first word
+        const bool node = held >= rows_k && nth >= 0 && nth < 32ll * a.words && (mask[nth >> 5] >> (nth & 31) & 1);
+        int from = 0, first_word = 0;
+        if (node && a.window) {
+            int depth = -1;
+            for (int w = 0; w < a.words; w++) depth += __popc(mask[w]);
+            from = (int)max(L0 + base + depth + 1ll - a.window, 0ll);
+            int drop = depth + 1 - a.window;   // of the words that it follows the window leaves the last ones
+            for (int w = 0; w < a.words && drop > 0; w++) {
+                unsigned bits = mask[w];
+                const int n = __popc(bits);
+                if (n < drop) {
+                    drop -= n;
+                    continue;
+                }
+                for (; drop > 0; drop--) {
+                    first_word = 32 * w + __ffs(bits);
+                    bits &= bits - 1;
+                }
+            }
+        }
+        int lo = node ? min(from, L0) : L0, hi = L0, sure = L0;
+        if constexpr (!SHARED) {
+            words_at = P + base;
+            lo = first_word ? words_at + first_word : from >= L0 ? P + (from - L0) : a.fused ? from : P;
+            hi = node ? P + held : lo;
+            sure = node ? words_at : 0;
+        }
+        if (wv == 0 && quad == 0) {
+            s.lo[c] = lo;
+            s.hi[c] = hi;
+        }
+        lo0 = min(lo0, lo);
+        lo1 = max(lo1, lo);
+        hi0 = min(hi0, sure);
+        hi1 = max(hi1, hi);
+    }
+    __syncthreads();
+    auto mn = [](int x, int y) { return min(x, y); };
+    auto mx = [](int x, int y) { return max(x, y); };
+    lo0 = __builtin_amdgcn_readfirstlane(over16(lo0, mn));
+    lo1 = __builtin_amdgcn_readfirstlane(over16(lo1, mx));
+    hi0 = __builtin_amdgcn_readfirstlane(over16(hi0, mn));
+    hi1 = __builtin_amdgcn_readfirstlane(over16(hi1, mx));
+    if constexpr (!SHARED) words_at = __builtin_amdgcn_readfirstlane(words_at);
+    // ---- the part: the first starts where the first column does; the last goes to the end ----
+    const int chunk = SHARED ? a.pchunk : a.ochunk;
+    const long long k0l = (long long)(lo0 & ~31) + (long long)part * chunk;
+    const int k1 = part + 1 == S ? hi1 : (int)min((long long)hi1, k0l + chunk);
+    const bool any = k0l < k1;
+    const int k0 = any ? (int)k0l : 0;
+
+    f32x4 o[E][NT];
+    // each column's reference, turned round (0 before there is one), its sum of weights and the score from which on it is rescaled
+    float nref[NT], l[NT], thr[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        thr[t] = -INFINITY;
+        nref[t] = l[t] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e][t] = f32x4{0, 0, 0, 0};
+    }
+    int kt = k0 + 32 * wv;
+    if (any && kt < k1) {
+        const int32_t* own = SHARED ? nullptr : a.table + (size_t)i * a.cols;
+        const int pl = a.page_log, pm = (1 << pl) - 1;
+        const size_t page_sz = ((size_t)a.n_kv << pl) * D, head_at = ((size_t)g << pl) * D;
+        // A block of 32 keys is two halves of 16, each in one page. Pages are whole, so that no key of theirs is out of reach; what
+        // lies behind the last one is masked
+        auto place_of = [&](int kt) { return SHARED || kt < P ? kt : kt - P; };
+        auto id_of = [&](int kt, int half) {
+            const bool in_shared = SHARED || kt < P;
+            const int last = in_shared ? L0 - 1 : hi1 - 1 - P;
+            return (in_shared ? a.prefix : own)[min(place_of(kt) + 16 * half, last) >> pl];
+        };
+        auto known = [&](int id) { return (unsigned)id < (unsigned)a.n_pages; };
+        // (in bytes; the same for the whole wave)
+        auto half_at = [&](int kt, int half, int id) {
+            return ((known(id) ? (size_t)id : 0) * page_sz + head_at + (size_t)((place_of(kt) + 16 * half) & pm) * D) * 2;
+        };
+        // whether every column sees every key of a block (of pages id0, id1)
+        auto is_full = [&](int kt, int id0, int id1) {
+            return kt >= lo1 && kt + 32 <= hi0 && (SHARED || kt < P ? L0 : hi1) - kt >= 32 && known(id0) && known(id1);
+        };
+        constexpr int RL = D / 8, RI = 64 / RL, KI = 32 / RI;  // lanes that load a row, rows that the wave loads at once
+        u32x4 kr[KI], kf[2][CH];
+        unsigned vw[8][VW];
+        const unsigned k_lane = lane * 16, v_lane = quad * (4 * D * 2) + m16 * (E * 2);
+        auto load_keys = [&](int kt, int id0, int id1) {
+#pragma unroll
+            for (int n = 0; n < KI; n++) {
+                const char* p = (const char*)a.keys + half_at(kt, n * RI / 16, n * RI / 16 ? id1 : id0) + (n * RI % 16) * (D * 2);
+                kr[n] = *(const u32x4*)(p + k_lane);
+            }
+        };
+        unsigned short* const kw = s.keys[wv] + lane / RL * (D + 8) + lane % RL * 8;
+        const unsigned short* const ks = s.keys[wv] + m16 * (D + 8) + quad * 8;
+        auto turn_keys = [&]() {
+#pragma unroll
+            for (int n = 0; n < KI; n++) *(u32x4*)(kw + n * RI * (D + 8)) = kr[n];
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int c = 0; c < CH; c++) kf[h][c] = *(const u32x4*)(ks + h * 16 * (D + 8) + c * 32);
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        };
+        auto load_values = [&](int kt, int id0, int id1) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const char* p = (const char*)a.values + half_at(kt, h, h ? id1 : id0);
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const char* q = p + v_lane + k * (D * 2);
+                    if constexpr (VW == 4) *(u32x4*)vw[4 * h + k] = *(const u32x4*)q;
+                    else if constexpr (VW == 2) *(uint2*)vw[4 * h + k] = *(const uint2*)q;
+                    else vw[4 * h + k][0] = *(const unsigned*)q;
+                }
+            }
+        };
+        auto scores = [&](int t, float (&x)[8]) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                f32x4 c4 = {0, 0, 0, 0};
+#pragma unroll
+                for (int c = 0; c < CH; c++) c4 = mat<T>::mul(kf[h][c], qf[c][t], c4);
+#pragma unroll
+                for (int r = 0; r < 4; r++) x[4 * h + r] = c4[r];
+            }
+        };
+        auto largest = [&](const float (&x)[8]) {      // (NaN where one is: the column is NaN then, whatever its reference)
+            float y = x[0];
+#pragma unroll
+            for (int k = 1; k < 8; k++) y = __builtin_elementwise_maximum(y, x[k]);
+            return y;
+        };
+        auto refer_to = [&](int t, float top) {
+            nref[t] = LIFT - top * a.c;
+            thr[t] = (SLACK + LIFT - nref[t]) / a.c;
+        };
+        // a column's new reference where its largest score passes the old one's slack
+        auto move_to = [&](int t, float top) {
+            const float y = over_quads(top);
+            if (y > thr[t]) {
+                const float old = nref[t];
+                const bool none = thr[t] == -INFINITY;
+                refer_to(t, y);
+                const float f = none ? 0.0f : exp2_(nref[t] - old);
+                l[t] *= f;
+#pragma unroll
+                for (int e = 0; e < E; e++) o[e][t] *= f;
+            }
+        };
+        unsigned pw[NT][4];
+        auto weights = [&](int t, float (&x)[8]) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                x[k] = exp2_(fmaf(x[k], a.c, nref[t]));
+                sum += x[k];
+            }
+            l[t] += sum;
+#pragma unroll
+            for (int k = 0; k < 4; k++) pw[t][k] = pack2<T>(x[2 * k], x[2 * k + 1]);
+        };
+        auto add_values = [&]() {
+#pragma unroll
+            for (int e = 0; e < E; e++) {  // dimension m16 * E + e of eight keys
+                const unsigned sel = (e & 1) ? 0x07060302u : 0x05040100u;
+                u32x4 vf;
+#pragma unroll
+                for (int k = 0; k < 4; k++) vf[k] = __builtin_amdgcn_perm(vw[2 * k + 1][e >> 1], vw[2 * k][e >> 1], sel);
+#pragma unroll
+                for (int t = 0; t < NT; t++) o[e][t] = mat<T>::mul(vf, u32x4{pw[t][0], pw[t][1], pw[t][2], pw[t][3]}, o[e][t]);
+            }
+        };
+        // of a lane's eight keys those that its column sees
+        auto sees = [&](int t, int kt, int id0, int id1) {
+            const bool in_shared = SHARED || kt < P;
+            const int c = 16 * t + m16, from = s.lo[c], stop = min(s.hi[c], in_shared ? L0 : hi1);
+            unsigned bits = 0;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int first = kt + 16 * h + quad * 4;
+                unsigned four = known(h ? id1 : id0) ? 0xFu : 0u;
+                if (!SHARED && !in_shared) four &= tree_bits(s.mask[c], a.words, first - words_at);
+                four &= from - first >= 4 ? 0u : 0xFu << max(from - first, 0);
+                bits |= (four & (stop <= first ? 0u : 0xFu >> max(4 - (stop - first), 0))) << (4 * h);
+            }
+            return bits;
+        };
+        bool odd = false;                  // infinities or NaN among values that some columns see
+        bool start = max(lo1, k0) + 128 <= min(hi0, k1) - 31;      // (each wave has a block that its columns see whole)
+#pragma unroll 1
+        for (int first = kt; first < k1; first += 63 * 128) {
+            // page ids of the wave's next 63 blocks, one a lane, and which of these blocks all columns see whole (the bit behind the
+            // last one's is not set)
+            const int many = min((k1 - first + 127) / 128, 63), lanes = first + 128 * min(lane, many - 1);
+            const int ids0 = id_of(lanes, 0), ids1 = id_of(lanes, 1);
+            const unsigned long long whole = __ballot(lane < many && is_full(lanes, ids0, ids1));
+            auto id = [&](int n, int half) { return __builtin_amdgcn_readlane(half ? ids1 : ids0, n); };
+            auto ask_keys = [&](int n) {
+                n = min(n, many - 1);
+                load_keys(first + 128 * n, id(n, 0), id(n, 1));
+            };
+            auto ask_values = [&](int n) {
+                n = min(n, many - 1);
+                load_values(first + 128 * n, id(n, 0), id(n, 1));
+            };
+            // (the order in which they are asked for is the one in which they are waited for)
+            ask_keys(0);
+            turn_keys();
+            ask_keys(1);
+            __builtin_amdgcn_sched_barrier(0);
+            ask_values(0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (start) {
+                // The first reference is the largest of all four waves' first blocks: far fewer scores pass it by the slack later on
+                start = false;
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    float x[8];
+                    scores(t, x);
+                    const float y = over_quads(largest(x));
+                    if (quad == 0) s.top[wv][16 * t + m16] = whole & 1 ? y : -INFINITY;
+                }
+                __syncthreads();
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    const int c = 16 * t + m16;
+                    const float y = fmaxf(fmaxf(s.top[0][c], s.top[1][c]), fmaxf(s.top[2][c], s.top[3][c]));
+                    if (y > -INFINITY) refer_to(t, y);
+                }
+            }
+            int n = 0;
+#pragma unroll 1
+            for (;;) {
+                // ---- blocks that all columns see whole ----
+#pragma unroll 1
+                while (whole >> n & 1) {
+                    float x[NT][8], top[NT];
+#pragma unroll
+                    for (int t = 0; t < NT; t++) scores(t, x[t]);
+                    turn_keys();
+                    ask_keys(n + 2);
+                    bool over = false;
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        top[t] = largest(x[t]);
+                        over |= top[t] > thr[t];
+                    }
+                    if (__any(over)) {
+#pragma unroll
+                        for (int t = 0; t < NT; t++) move_to(t, top[t]);
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; t++) weights(t, x[t]);
+                    add_values();
+                    ask_values(++n);
+                }
+                if (n >= many) break;
+                // ---- others: at a window's edges, the shared positions' end, pages that are not there, and the tree ----
+                unsigned any_sees = 0;
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    const unsigned bits = sees(t, first + 128 * n, id(n, 0), id(n, 1));
+                    any_sees |= bits;
+                    float x[8];
+                    scores(t, x);
+#pragma unroll
+                    for (int k = 0; k < 8; k++) x[k] = bits >> k & 1 ? x[k] : -INFINITY;
+                    const float top = largest(x);
+                    if (__any(top > thr[t])) move_to(t, top);
+                    weights(t, x);
+                }
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) any_sees |= __shfl_xor(any_sees, o);
+                // A weight of 0 times an infinity would reach columns that do not see the key: such values are left out (below)
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+#pragma unroll
+                    for (int w = 0; w < VW; w++) {
+                        const unsigned v = any_sees >> k & 1 ? vw[k][w] : 0u;
+                        const bool bad0 = (v & mat<T>::EXP) == mat<T>::EXP, bad1 = (v >> 16 & mat<T>::EXP) == mat<T>::EXP;
+                        odd |= bad0 || bad1;
+                        vw[k][w] = v & ((bad0 ? 0u : 0xFFFFu) | (bad1 ? 0u : 0xFFFF0000u));
+                    }
+                add_values();
+                turn_keys();
+                ask_keys(n + 2);
+                ask_values(++n);
+                if (n >= many) break;
+                }
+        }
+        if (__any(odd)) {
+            // Infinities and NaN that some columns of a block see: how many a column sees of either sign (NaN: of both, and so an
+            // infinity whose weight is 0) is counted by products of ones
+#pragma unroll 1
+            for (kt = k0 + 32 * wv; kt < k1; kt += 128) {
+                const int id0 = id_of(kt, 0), id1 = id_of(kt, 1);
+                if (is_full(kt, id0, id1)) continue;
+                load_keys(kt, id0, id1);
+                load_values(kt, id0, id1);
+                turn_keys();
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    const unsigned bits = sees(t, kt, id0, id1);
+                    float x[8];
+                    scores(t, x);
+                    u32x4 st, nt;              // ones for the keys that the column sees, and for those of them without weight
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const unsigned w = pack2<T>(exp2_(fmaf(x[2 * k], a.c, nref[t])), exp2_(fmaf(x[2 * k + 1], a.c, nref[t])));
+                        st[k] = (bits >> 2 * k & 1 ? mat<T>::ONE : 0u) | (bits >> 2 * k & 2 ? mat<T>::ONE << 16 : 0u);
+                        nt[k] = st[k] & ((w & 0x7FFFu ? 0u : 0xFFFFu) | (w & 0x7FFF0000u ? 0u : 0xFFFF0000u));
+                    }
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        u32x4 up, down;
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            up[k] = down[k] = 0;
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                const unsigned v = vw[2 * k + h][e >> 1] >> (16 * (e & 1)) & 0xFFFFu, one = mat<T>::ONE << (16 * h);
+                                const bool bad = (v & mat<T>::EXP) == mat<T>::EXP, nan = bad && (v & (0x7FFFu ^ mat<T>::EXP));
+                                up[k] |= nan || (bad && !(v & 0x8000u)) ? one : 0u;
+                                down[k] |= nan || (bad && (v & 0x8000u)) ? one : 0u;
+                            }
+                        }
+                        const f32x4 plus = mat<T>::mul(down, nt, mat<T>::mul(up, st, f32x4{0, 0, 0, 0}));
+                        const f32x4 less = mat<T>::mul(up, nt, mat<T>::mul(down, st, f32x4{0, 0, 0, 0}));
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            if (plus[r] > 0.0f) o[e][t][r] += INFINITY;
+                            if (less[r] > 0.0f) o[e][t][r] -= INFINITY;
+                        }
+                    }
+                }
+            }
+        }
+    }
+    float m[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) m[t] = thr[t] == -INFINITY ? -INFINITY : -nref[t];
+    __syncthreads();                       // (their keys' space is the join's)
+    // ---- the four waves joined: 2 and 3 into 0 and 1, then 1 into 0 ----
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        l[t] += __shfl_xor(l[t], 16);
+        l[t] += __shfl_xor(l[t], 32);
+    }
+#pragma unroll
+    for (int step = 2; step > 0; step >>= 1) {
+        if (k0 + 32 * step >= k1) continue;   // (waves from `step` on had no block)
+        if (wv >= step && wv < 2 * step) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const int c = 16 * t + m16;
+                if (quad == 0) {
+                    js.m[wv - step][c] = m[t];
+                    js.l[wv - step][c] = l[t];
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int e = 0; e < E; e++) js.o[wv - step][c * PITCH + (quad * 4 + r) * E + e] = o[e][t][r];
+            }
+        }
+        __syncthreads();
+        if (wv < step) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const int c = 16 * t + m16;
+                const float m2 = js.m[wv][c], l2 = js.l[wv][c];
+                const float to = fmaxf(m[t], m2), f1 = rescale(m[t], to), f2 = rescale(m2, to);
+                m[t] = to;
+                l[t] = l[t] * f1 + l2 * f2;
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+                        o[e][t][r] = o[e][t][r] * f1 + js.o[wv][c * PITCH + (quad * 4 + r) * E + e] * f2;
+            }
+        }
+        __syncthreads();
+    }
+    if (wv) return;
+    const bool alone = a.sp + a.so == 1;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const int c = 16 * t + m16;
+        if (c0 + c >= ncol) continue;
+        const size_t rh = (size_t)row_of(c) * a.n_head + head_of(c);
+        if (alone) {
+            float f = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+            if (a.gate) f *= 1.0f / (1.0f + expf(-a.gate[rh]));
+            unsigned* dst = (unsigned*)((T*)a.out + rh * D + quad * 4 * E);
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int e = 0; e < E; e += 2) {
+                    const float x = o[e][t][r], y = o[e + 1][t][r];
+                    dst[(r * E + e) / 2] = l[t] == 0.0f ? 0u : pack2<T>(x * f, y * f);
+                }
+            if (a.lse && quad == 0) a.lse[rh] = l[t] == 0.0f ? -INFINITY : (m[t] + log2f(l[t])) * 0.69314718055994531f;
+        } else {
+            const size_t at = (size_t)(SHARED ? part : a.sp + part) * a.rows * a.n_head + rh;
+            if (quad == 0) a.part_ml[at] = make_float2(m[t], l[t]);
+            if (any) {
+                float* dst = a.part_o + at * D + quad * 4 * E;
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int e = 0; e < E; e++) dst[r * E + e] = o[e][t][r];
+            }
+        }
+    }
+}
+
 constexpr int waves_of(int D, int nts, int nto) { return nts > 1 || nto > 1 ? 2 : D > 64 ? 3 : 4; }
 
 template <class T, int D, int NTS, int NTO>
 __global__ __launch_bounds__(256, waves_of(D, NTS, NTO)) void k_tree_attn(pattn_args a) {
-    __shared__ __align__(16) union { join_space<D, NTO> own; join_space<D, NTS ? NTS : 1> shared; } js;
+    __shared__ __align__(16) union { tree_space<D, NTO> own; tree_space<D, NTS ? NTS : 1> shared; } s;
     int b = blockIdx.x;
     if constexpr (NTS > 0) {
         const long long grp = b >> 3, gs = (a.shared_blocks + 7) >> 3, all = gridDim.x >> 3;
         const long long before = grp * gs / all, next = (grp + 1) * gs / all;   // shared groups before this one, with it
         if (next > before) {
             b = (int)(before * 8) + (b & 7);
-            if (b < a.shared_blocks) attend<T, D, NTS ? NTS : 1, true, true>(a, b, js.shared);
+            if (b < a.shared_blocks) attend<T, D, NTS ? NTS : 1, true>(a, b, s.shared);
             return;
         }
         b = (int)((grp - before) * 8) + (b & 7);
         if (b >= a.own_blocks) return;
     }
-    attend<T, D, NTO, false, true>(a, b, js.own);
+    attend<T, D, NTO, false>(a, b, s.own);
 }
 
 template <class T, int D, int NTS, int NTO> hipError_t run_attn(const pattn_args& a, hipStream_t s) {
@@ -44,6 +586,40 @@ template <class T> hipError_t run_dim(int D, const pattn_args& a, hipStream_t s)
 }
 
 }  // namespace
+
+// Which workgroups take the shared positions, and into how many parts the keys go.
+bool tree_attn_split(int D, pattn_args& a) {
+    const int nto = 16 * attn_col_groups(D, (long long)a.max_rows * a.grp), nts = 16 * attn_col_groups(D, (long long)a.rows * a.grp);
+    const long long cols = (long long)a.rows * a.grp, own = cols / nto + a.n, all = (cols + nts - 1) / nts;
+    auto split = [&](long long tiles, long long range, long long want, int* parts, int* chunk) {
+        const long long p = std::max(std::min(want / std::max(tiles * a.n_kv, 1ll), (range + 255) / 256), 1ll);
+        *chunk = (int)std::max(((range + p - 1) / p + 127) / 128 * 128, 128ll);
+        *parts = (int)std::max((range + *chunk - 1) / *chunk, 1ll);
+    };
+    a.own_at = (a.prefix_len + 31) / 32 * 32;
+    // Requests read the shared positions themselves where their columns fill their workgroups (sharing would save no reads, and
+    // nothing has to be joined), and where they are few or the shared positions are: sharing costs a launch and the parts' sums.
+    // us apart and fused, by requests x words behind shared positions, 1000 own ones: 8 kv heads of 64: 64 x 64 behind 1024 151
+    // and 92, 64 x 24 behind 4096 113 and 112; with more than twice as many tiles of requests as of all columns 8 x 4 behind 4096 23 and
+    // 18 (tiles times positions 49152), 64 x 4 behind 1024 35 and 25 (98304), 32 x 2 behind 4096 29 and 33 (163840), 64 x 8
+    // behind 4096 59 and 88 (327680). 4 of 128, whose tiles are half as wide: up to three times as many tiles 32 x 8 behind 1024 32 and 26
+    // (49152), 64 x 8 behind 4096 48 and 58 (393216), above 8 x 4 behind 256 15.7 and 16.5 (3072), behind 1024 16.3 and 18.6
+    a.fused = a.prefix_len == 0 || own <= all * 2 || own * a.prefix_len <= (D <= 64 ? 100000 : own <= all * 3 ? 200000 : 4096);
+    a.sp = a.pchunk = 0;
+    if (!a.fused) split(all, a.window && a.window + 31ll < a.prefix_len ? a.window + 31ll : a.prefix_len, 512, &a.sp, &a.pchunk);
+    long long range = (a.fused ? a.own_at : 0ll) + a.max_len;
+    if (a.window) range = std::min(range, a.window + 63ll + a.max_rows);
+    // One and a half workgroups per compute unit, of 256 keys or more: one request of up to 32749 positions and 33 words (4 kv heads of
+    // 128) 28 to 29 us, with half as many parts 35, with twice as many 46 (the join reads all of them)
+    split((cols + nto - 1) / nto, range, 384, &a.so, &a.ochunk);
+    const long long shared_blocks = all * a.n_kv * a.sp, own_blocks = own * a.n_kv * a.so;
+    const long long rh = (long long)a.rows * a.n_head, join = a.sp + a.so == 1 ? 0 : a.sp + a.so > 16 ? rh : (rh + 3) / 4;
+    // (columns of one kv head are counted in 32 bits in the kernel)
+    if (shared_blocks + own_blocks + 16 > most_blocks(256) || join > most_blocks(256) || cols > INT_MAX / 2) return false;
+    a.shared_blocks = (int)shared_blocks;
+    a.own_blocks = (int)own_blocks;
+    return true;
+}
 
 hipError_t launch_tree_attn(int D, int type, const pattn_args& a, hipStream_t s) {
     const hipError_t e = type == TY_F16 ? run_dim<_Float16>(D, a, s) : run_dim<__bf16>(D, a, s);

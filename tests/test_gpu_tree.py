@@ -188,7 +188,8 @@ def tree_reference(c):
             out[r] = (e / e.sum(0))[..., None].mul(v).sum(0)
             off = 2.0 ** -24 * (D * size + 3 * s.abs().amax(0) / math.log(2) + len(seen) / 128 + 16) + 2.0 ** -20
             tol_lse[r] = off + 2.0 ** -23 * lse[r].abs()
-            under = 2.0 ** -36 * len(seen) if c["kind"] == "f16" else 0.0
+            # (f16 weights are 2^8 of the running maximum's: below 2^-14 their places are 2^-24 apart)
+            under = 2.0 ** -33 * len(seen) if c["kind"] == "f16" else 0.0
             tol[r, :, 0] = (HALF[c["kind"]] * 1.01 + under + 2 * off) * v.abs().amax(0).amax(-1)
         r0 += m
     if c["gate"] is not None:
@@ -247,6 +248,26 @@ def test_attn_largest_trees(ctx, kind, D, H, K):
 @pytest.mark.parametrize("n,length,prefix,m", [(1, 3000, 0, 9), (2, 1111, 2500, 33), (30, 300, 1100, 5), (1, 9000, 100, 2)])
 def test_attn_many_parts(ctx, n, length, prefix, m):
     check_tree(ctx, tree_case(n, [length - 7 * i for i in range(n)], [m] * n, 4, 2, 64, 64, "f16", prefix=prefix))
+
+
+def test_attn_long_parts(ctx):
+    """Requests that are one part each, of lengths on either side of a whole number of a wave's page lookups (63 blocks of 128
+    keys): single words, against the attention of single rows."""
+    K, D, page, lens = 8, 32, 128, [8063, 8064, 8065, 8066, 8191, 8192, 8193, 16127, 16128, 16129, 17000] * 7
+    g = torch.Generator().manual_seed(8)
+    pages, n = -(-max(lens) // page), len(lens)
+    keys, values = (torch.randn(pages, K, page, D, generator=g).half().cuda() for _ in range(2))
+    q = torch.randn(n, K, D, generator=g).half().cuda()
+    shape = nunchi_amd.PageShape(K, K, D, page, pages)
+    table, length = torch.randperm(pages, generator=g).int().repeat(n, 1).cuda(), i32(lens)
+    out = [torch.zeros_like(q) for _ in range(2)]
+    lse = [torch.zeros(n, K, device="cuda") for _ in range(2)]
+    works = [torch.empty(f, dtype=torch.uint8, device="cuda") for f in (nunchi_amd.page_attn_work(shape, n, n, max(lens)), nunchi_amd.tree_attn_work(shape, n, n, max(lens), 1))]
+    nunchi_amd.page_attn(ctx, shape, q, keys, values, table, length, out[0], works[0], max(lens), lse=lse[0])
+    nunchi_amd.tree_attn(ctx, shape, q, keys, values, table, length, i32(range(n + 1)), i32([[1]] * n), out[1], works[1], max(lens), 1, lse=lse[1])
+    # (both within half a step of the largest value and of the result; scores of 32 products below 32 in size)
+    assert ((out[0].float() - out[1].float()).abs() <= 2 * HALF["f16"] * (5.5 + out[0].float().abs())).all()
+    assert ((lse[0] - lse[1]).abs() <= 2 * (2.0 ** -24 * (32 * 32 + 140) + 2.0 ** -20 + 2.0 ** -23 * lse[0].abs())).all()
 
 
 def test_attn_masks_that_are_no_trees(ctx):
