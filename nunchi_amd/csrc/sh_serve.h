@@ -54,7 +54,7 @@ struct pattn_args {
     float2* part_ml;           // [sp + so][rows][n_head] maximum (powers of two) and sum of weights
     // trees of drafted words alone: which words of its request a row sees
     const unsigned* mask;      // [rows][words]
-    int words;
+    int words, nts, nto;       // words of a mask; column groups of a workgroup of the shared positions and of the own ones
 };
 
 struct sample_args {

@@ -32,6 +32,22 @@ __device__ __forceinline__ unsigned tree_bits(const unsigned* mask, int words, i
     return (unsigned)(two >> (from & 31)) & 0xFu;
 }
 
+// the largest of the wave's first 16 lanes
+__device__ __forceinline__ int most_of_16(int x) {
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x128, 0xF, 0xF, false));   // row_ror:8, 4, 2, 1
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x124, 0xF, 0xF, false));
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x122, 0xF, 0xF, false));
+    x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x121, 0xF, 0xF, false));
+    return __builtin_amdgcn_readfirstlane(x);
+}
+// the bits of a lane's 16
+__device__ __forceinline__ unsigned any_of_16(unsigned x) {
+    x |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xF, 0xF, false);
+    x |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xF, 0xF, false);
+    x |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xF, 0xF, false);
+    x |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xF, 0xF, false);
+    return x;
+}
 // the largest of four lanes 16 apart
 __device__ __forceinline__ float over_quads(float x) {
     const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -40,20 +56,26 @@ __device__ __forceinline__ float over_quads(float x) {
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// The last request k with f(cu[k], k) <= at (f(cu[0], 0) <= at, f does not fall), its row starts and its length: a wave looks at
-// 64 requests at a time.
-struct found_request {
-    int k, cu0, cu1, len;
+// A request, its row starts and its length, and which of its tiles of columns a workgroup takes.
+struct tile_of_request {
+    int k, cu0, cu1, len, tile;
 };
-template <class F> __device__ __forceinline__ found_request find_request(const pattn_args& a, int at, int lane, F f) {
+
+// Tile `at` of all requests': request k has the tiles first(k) .. first(k + 1) - 1, at least as many as its columns fill. A wave
+// looks at 63 requests at a time. (Longest requests first, so that the last workgroups to start are the shortest: no gain.)
+__device__ __forceinline__ tile_of_request find_tile(const pattn_args& a, int at, int lane, int nc) {
+    auto row_at = [&](int cu) { return min(max(cu, 0), a.rows); };
+    auto first = [&](int cu, int k) { return (int)((long long)row_at(cu) * a.grp / nc) + k; };
     int lo = 0, hi = a.n;
     for (;;) {
         const int step = (hi - lo + 62) / 63, k = lo + lane * step;
         const int cu = a.cu[min(k, a.n)], len = a.len[min(k, a.n - 1)];
-        const int there = max(__popcll(__ballot(k < hi && f(cu, k) <= at)), 1);
+        const int there = max(__popcll(__ballot(k < hi && first(cu, k) <= at)), 1);
         lo += (there - 1) * step;
-        if (step == 1)
-            return {lo, __builtin_amdgcn_readlane(cu, there - 1), __builtin_amdgcn_readlane(cu, there), __builtin_amdgcn_readlane(len, there - 1)};
+        if (step == 1) {
+            const int cu0 = __builtin_amdgcn_readlane(cu, there - 1);
+            return {lo, cu0, __builtin_amdgcn_readlane(cu, there), __builtin_amdgcn_readlane(len, there - 1), at - first(cu0, lo)};
+        }
         hi = min(hi, lo + step);
     }
 }
@@ -85,26 +107,31 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
     const int tile = block / per;
     // ---- the workgroup's columns ----
     int i = 0, r0 = 0, r1, ct = tile;      // request, its rows, tile of columns within them
-    [[maybe_unused]] found_request mine{};
+    [[maybe_unused]] tile_of_request mine{};
     if constexpr (SHARED) {
         r1 = min(max(a.cu[a.n], 0), a.rows);
     } else {
-        // request i owns the tiles first(i) .. first(i + 1) - 1, at least as many as its columns fill
-        auto row_at = [&](int cu) { return min(max(cu, 0), a.rows); };
-        auto first = [&](int cu, int k) { return (int)((long long)row_at(cu) * a.grp / NC) + k; };
-        mine = find_request(a, tile, lane, first);
+        mine = find_tile(a, tile, lane, NC);
         i = mine.k;
-        ct = tile - first(mine.cu0, i);
-        r0 = row_at(mine.cu0);
-        r1 = min(row_at(mine.cu1), r0 + a.max_rows);
+        ct = mine.tile;
+        r0 = min(max(mine.cu0, 0), a.rows);
+        r1 = min(min(max(mine.cu1, 0), a.rows), r0 + a.max_rows);
     }
     const int ncol = (r1 - r0) * a.grp, c0 = ct * NC;
     if (c0 < 0 || c0 >= ncol) return;
-    auto row_of = [&](int c) { return r0 + min(c0 + c, ncol - 1) / a.grp; };
-    auto head_of = [&](int c) { return g * a.grp + min(c0 + c, ncol - 1) % a.grp; };
-    for (int k = threadIdx.x; k < NC * (a.words + 1); k += 256) {
-        const int c = k / (a.words + 1), w = k - c * (a.words + 1);
-        s.mask[c][w] = w < a.words ? a.mask[(size_t)row_of(c) * a.words + w] : 0u;
+    // (a column's row and head: within a tile small numbers are divided)
+    const int row0 = c0 / a.grp, over0 = c0 - row0 * a.grp, last = ncol - 1 - c0, by = a.grp < 64 ? 65536 / a.grp + 1 : 0;
+    auto rows_on = [&](int c) {
+        const int x = over0 + min(c, last);
+        return a.grp < 64 ? (x * by) >> 16 : x >= a.grp ? 1 : 0;
+    };
+    auto row_of = [&](int c) { return r0 + row0 + rows_on(c); };
+    auto head_of = [&](int c) { return g * a.grp + over0 + min(c, last) - rows_on(c) * a.grp; };
+    {
+        constexpr int PER = 256 / NC;      // threads a column
+        const int c = threadIdx.x / PER;
+        const unsigned* from = a.mask + (size_t)row_of(c) * a.words;
+        for (int w = threadIdx.x % PER; w <= a.words; w += PER) s.mask[c][w] = w < a.words ? from[w] : 0u;
     }
     u32x4 qf[CH][NT];
 #pragma unroll
@@ -163,12 +190,10 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
         hi1 = max(hi1, hi);
     }
     __syncthreads();
-    auto mn = [](int x, int y) { return min(x, y); };
-    auto mx = [](int x, int y) { return max(x, y); };
-    lo0 = __builtin_amdgcn_readfirstlane(over16(lo0, mn));
-    lo1 = __builtin_amdgcn_readfirstlane(over16(lo1, mx));
-    hi0 = __builtin_amdgcn_readfirstlane(over16(hi0, mn));
-    hi1 = __builtin_amdgcn_readfirstlane(over16(hi1, mx));
+    lo0 = -most_of_16(-lo0);
+    lo1 = most_of_16(lo1);
+    hi0 = -most_of_16(-hi0);
+    hi1 = most_of_16(hi1);
     if constexpr (!SHARED) words_at = __builtin_amdgcn_readfirstlane(words_at);
     // ---- the part: the first starts where the first column does; the last goes to the end ----
     const int chunk = SHARED ? a.pchunk : a.ochunk;
@@ -191,7 +216,6 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
     if (any && kt < k1) {
         const int32_t* own = SHARED ? nullptr : a.table + (size_t)i * a.cols;
         const int pl = a.page_log, pm = (1 << pl) - 1;
-        const size_t page_sz = ((size_t)a.n_kv << pl) * D, head_at = ((size_t)g << pl) * D;
         // A block of 32 keys is two halves of 16, each in one page. Pages are whole, so that no key of theirs is out of reach; what
         // lies behind the last one is masked
         auto place_of = [&](int kt) { return SHARED || kt < P ? kt : kt - P; };
@@ -201,9 +225,9 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
             return (in_shared ? a.prefix : own)[min(place_of(kt) + 16 * half, last) >> pl];
         };
         auto known = [&](int id) { return (unsigned)id < (unsigned)a.n_pages; };
-        // (in bytes; the same for the whole wave)
-        auto half_at = [&](int kt, int half, int id) {
-            return ((known(id) ? (size_t)id : 0) * page_sz + head_at + (size_t)((place_of(kt) + 16 * half) & pm) * D) * 2;
+        // a half's place in the cache, counted in halves (of 1 KB and more: 32 bits reach 4 TB)
+        auto half_of = [&](int kt, int half, int id) {
+            return ((known(id) ? (unsigned)id : 0u) * (unsigned)a.n_kv + (unsigned)g) * (unsigned)((pm + 1) >> 4) + (unsigned)(((place_of(kt) + 16 * half) & pm) >> 4);
         };
         // whether every column sees every key of a block (of pages id0, id1)
         auto is_full = [&](int kt, int id0, int id1) {
@@ -213,10 +237,10 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
         u32x4 kr[KI], kf[2][CH];
         unsigned vw[8][VW];
         const unsigned k_lane = lane * 16, v_lane = quad * (4 * D * 2) + m16 * (E * 2);
-        auto load_keys = [&](int kt, int id0, int id1) {
+        auto load_keys = [&](unsigned half0, unsigned half1) {
 #pragma unroll
             for (int n = 0; n < KI; n++) {
-                const char* p = (const char*)a.keys + half_at(kt, n * RI / 16, n * RI / 16 ? id1 : id0) + (n * RI % 16) * (D * 2);
+                const char* p = (const char*)a.keys + (size_t)(n * RI / 16 ? half1 : half0) * (32 * D) + (n * RI % 16) * (D * 2);
                 kr[n] = *(const u32x4*)(p + k_lane);
             }
         };
@@ -236,10 +260,10 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         };
-        auto load_values = [&](int kt, int id0, int id1) {
+        auto load_values = [&](unsigned half0, unsigned half1) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const char* p = (const char*)a.values + half_at(kt, h, h ? id1 : id0);
+                const char* p = (const char*)a.values + (size_t)(h ? half1 : half0) * (32 * D);
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const char* q = p + v_lane + k * (D * 2);
@@ -294,16 +318,18 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
 #pragma unroll
             for (int k = 0; k < 4; k++) pw[t][k] = pack2<T>(x[2 * k], x[2 * k + 1]);
         };
-        auto add_values = [&]() {
+        u32x4 vf[E];
+        auto turn_values = [&]() {
 #pragma unroll
             for (int e = 0; e < E; e++) {  // dimension m16 * E + e of eight keys
                 const unsigned sel = (e & 1) ? 0x07060302u : 0x05040100u;
-                u32x4 vf;
 #pragma unroll
-                for (int k = 0; k < 4; k++) vf[k] = __builtin_amdgcn_perm(vw[2 * k + 1][e >> 1], vw[2 * k][e >> 1], sel);
-#pragma unroll
-                for (int t = 0; t < NT; t++) o[e][t] = mat<T>::mul(vf, u32x4{pw[t][0], pw[t][1], pw[t][2], pw[t][3]}, o[e][t]);
+                for (int k = 0; k < 4; k++) vf[e][k] = __builtin_amdgcn_perm(vw[2 * k + 1][e >> 1], vw[2 * k][e >> 1], sel);
             }
+        };
+        auto add_values = [&](int t) {
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e][t] = mat<T>::mul(vf[e], u32x4{pw[t][0], pw[t][1], pw[t][2], pw[t][3]}, o[e][t]);
         };
         // of a lane's eight keys those that its column sees
         auto sees = [&](int t, int kt, int id0, int id1) {
@@ -329,15 +355,10 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
             const int many = min((k1 - first + 127) / 128, 63), lanes = first + 128 * min(lane, many - 1);
             const int ids0 = id_of(lanes, 0), ids1 = id_of(lanes, 1);
             const unsigned long long whole = __ballot(lane < many && is_full(lanes, ids0, ids1));
-            auto id = [&](int n, int half) { return __builtin_amdgcn_readlane(half ? ids1 : ids0, n); };
-            auto ask_keys = [&](int n) {
-                n = min(n, many - 1);
-                load_keys(first + 128 * n, id(n, 0), id(n, 1));
-            };
-            auto ask_values = [&](int n) {
-                n = min(n, many - 1);
-                load_values(first + 128 * n, id(n, 0), id(n, 1));
-            };
+            const unsigned halves0 = half_of(lanes, 0, ids0), halves1 = half_of(lanes, 1, ids1);
+            // (behind the last block it is asked for again)
+            auto ask_keys = [&](int n) { load_keys(__builtin_amdgcn_readlane(halves0, min(n, many - 1)), __builtin_amdgcn_readlane(halves1, min(n, many - 1))); };
+            auto ask_values = [&](int n) { load_values(__builtin_amdgcn_readlane(halves0, min(n, many - 1)), __builtin_amdgcn_readlane(halves1, min(n, many - 1))); };
             // (the order in which they are asked for is the one in which they are waited for)
             ask_keys(0);
             turn_keys();
@@ -384,54 +405,72 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
 #pragma unroll
                         for (int t = 0; t < NT; t++) move_to(t, top[t]);
                     }
+                    // products of a column group with the values beside the next group's weights
+                    weights(0, x[0]);
+                    turn_values();
 #pragma unroll
-                    for (int t = 0; t < NT; t++) weights(t, x[t]);
-                    add_values();
+                    for (int t = 0; t < NT; t++) {
+                        add_values(t);
+                        if (t + 1 < NT) weights(t + 1, x[t + 1]);
+                    }
                     ask_values(++n);
                 }
                 if (n >= many) break;
                 // ---- others: at a window's edges, the shared positions' end, pages that are not there, and the tree ----
-                unsigned any_sees = 0;
+                unsigned any_sees = 0, bits[NT];
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    const unsigned bits = sees(t, first + 128 * n, id(n, 0), id(n, 1));
-                    any_sees |= bits;
+                    bits[t] = sees(t, first + 128 * n, __builtin_amdgcn_readlane(ids0, n), __builtin_amdgcn_readlane(ids1, n));
+                    any_sees |= bits[t];
+                }
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
                     float x[8];
                     scores(t, x);
 #pragma unroll
-                    for (int k = 0; k < 8; k++) x[k] = bits >> k & 1 ? x[k] : -INFINITY;
+                    for (int k = 0; k < 8; k++) x[k] = bits[t] >> k & 1 ? x[k] : -INFINITY;
                     const float top = largest(x);
                     if (__any(top > thr[t])) move_to(t, top);
                     weights(t, x);
                 }
-#pragma unroll
-                for (int o = 8; o > 0; o >>= 1) any_sees |= __shfl_xor(any_sees, o);
-                // A weight of 0 times an infinity would reach columns that do not see the key: such values are left out (below)
+                any_sees = any_of_16(any_sees);
+                unsigned full = 0;             // (a value whose exponent bits are all set carries into its sign)
 #pragma unroll
                 for (int k = 0; k < 8; k++)
 #pragma unroll
                     for (int w = 0; w < VW; w++) {
-                        const unsigned v = any_sees >> k & 1 ? vw[k][w] : 0u;
-                        const bool bad0 = (v & mat<T>::EXP) == mat<T>::EXP, bad1 = (v >> 16 & mat<T>::EXP) == mat<T>::EXP;
-                        odd |= bad0 || bad1;
-                        vw[k][w] = v & ((bad0 ? 0u : 0xFFFFu) | (bad1 ? 0u : 0xFFFF0000u));
+                        vw[k][w] &= 0u - (any_sees >> k & 1);
+                        full |= (vw[k][w] & mat<T>::EXP * 0x10001u) + (mat<T>::EXP & -mat<T>::EXP) * 0x10001u;
                     }
-                add_values();
+                if (__any(full & 0x80008000u)) {
+                    // A weight of 0 times an infinity would reach columns that do not see the key: such values are left out (below)
+                    odd = true;
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+#pragma unroll
+                        for (int w = 0; w < VW; w++) {
+                            if ((vw[k][w] & mat<T>::EXP) == mat<T>::EXP) vw[k][w] &= 0xFFFF0000u;
+                            if ((vw[k][w] >> 16 & mat<T>::EXP) == mat<T>::EXP) vw[k][w] &= 0x0000FFFFu;
+                        }
+                }
+                turn_values();
+#pragma unroll
+                for (int t = 0; t < NT; t++) add_values(t);
                 turn_keys();
                 ask_keys(n + 2);
                 ask_values(++n);
                 if (n >= many) break;
                 }
         }
-        if (__any(odd)) {
+        if (odd) {
             // Infinities and NaN that some columns of a block see: how many a column sees of either sign (NaN: of both, and so an
             // infinity whose weight is 0) is counted by products of ones
 #pragma unroll 1
             for (kt = k0 + 32 * wv; kt < k1; kt += 128) {
                 const int id0 = id_of(kt, 0), id1 = id_of(kt, 1);
                 if (is_full(kt, id0, id1)) continue;
-                load_keys(kt, id0, id1);
-                load_values(kt, id0, id1);
+                load_keys(half_of(kt, 0, id0), half_of(kt, 1, id1));
+                load_values(half_of(kt, 0, id0), half_of(kt, 1, id1));
                 turn_keys();
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
@@ -474,6 +513,13 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
     float m[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) m[t] = thr[t] == -INFINITY ? -INFINITY : -nref[t];
+    const bool alone = a.sp + a.so == 1;
+    float gate[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const int c = 16 * t + m16;
+        gate[t] = alone && a.gate && wv == 0 ? a.gate[(size_t)row_of(c) * a.n_head + head_of(c)] : INFINITY;
+    }
     __syncthreads();                       // (their keys' space is the join's)
     // ---- the four waves joined: 2 and 3 into 0 and 1, then 1 into 0 ----
 #pragma unroll
@@ -493,9 +539,7 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
                     js.l[wv - step][c] = l[t];
                 }
 #pragma unroll
-                for (int r = 0; r < 4; r++)
-#pragma unroll
-                    for (int e = 0; e < E; e++) js.o[wv - step][c * PITCH + (quad * 4 + r) * E + e] = o[e][t][r];
+                for (int e = 0; e < E; e++) *(f32x4*)(js.o[wv - step] + c * PITCH + quad * 4 * E + e * 4) = o[e][t];
             }
         }
         __syncthreads();
@@ -508,16 +552,12 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
                 m[t] = to;
                 l[t] = l[t] * f1 + l2 * f2;
 #pragma unroll
-                for (int r = 0; r < 4; r++)
-#pragma unroll
-                    for (int e = 0; e < E; e++)
-                        o[e][t][r] = o[e][t][r] * f1 + js.o[wv][c * PITCH + (quad * 4 + r) * E + e] * f2;
+                for (int e = 0; e < E; e++) o[e][t] = o[e][t] * f1 + *(const f32x4*)(js.o[wv] + c * PITCH + quad * 4 * E + e * 4) * f2;
             }
         }
         __syncthreads();
     }
     if (wv) return;
-    const bool alone = a.sp + a.so == 1;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
         const int c = 16 * t + m16;
@@ -525,7 +565,7 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
         const size_t rh = (size_t)row_of(c) * a.n_head + head_of(c);
         if (alone) {
             float f = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
-            if (a.gate) f *= 1.0f / (1.0f + expf(-a.gate[rh]));
+            f *= 1.0f / (1.0f + expf(-gate[t]));       // (no gate: 1)
             unsigned* dst = (unsigned*)((T*)a.out + rh * D + quad * 4 * E);
 #pragma unroll
             for (int r = 0; r < 4; r++)
@@ -549,7 +589,11 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
     }
 }
 
-constexpr int waves_of(int D, int nts, int nto) { return nts > 1 || nto > 1 ? 2 : D > 64 ? 3 : 4; }
+// waves per SIMD that the registers are to allow
+constexpr int waves_of(int D, int nts, int nto) {
+    const int nt = nts > nto ? nts : nto;
+    return nt == 4 || (nt == 2 && D > 64) ? 2 : nt == 2 || D > 64 ? 3 : 4;
+}
 
 template <class T, int D, int NTS, int NTO>
 __global__ __launch_bounds__(256, waves_of(D, NTS, NTO)) void k_tree_attn(pattn_args a) {
@@ -575,11 +619,10 @@ template <class T, int D, int NTS, int NTO> hipError_t run_attn(const pattn_args
     return hipGetLastError();
 }
 template <class T, int D> hipError_t run_all(const pattn_args& a, hipStream_t s) {
-    constexpr int M = attn_many(D);
-    const int nts = a.sp ? attn_col_groups(D, (long long)a.rows * a.grp) : 0, nto = attn_col_groups(D, (long long)a.max_rows * a.grp);
-    if (nts == 0) return nto == 1 ? run_attn<T, D, 0, 1>(a, s) : run_attn<T, D, 0, M>(a, s);
-    if (nts == 1) return run_attn<T, D, 1, 1>(a, s);   // (a request has no more columns than all of them)
-    return nto == 1 ? run_attn<T, D, M, 1>(a, s) : run_attn<T, D, M, M>(a, s);
+    if (a.sp) return a.nts == 1 ? run_attn<T, D, 1, 1>(a, s) : a.nto == 1 ? run_attn<T, D, 2, 1>(a, s) : run_attn<T, D, 2, 2>(a, s);
+    if constexpr (D <= 64)
+        if (a.nto == 4) return run_attn<T, D, 0, 4>(a, s);
+    return a.nto == 1 ? run_attn<T, D, 0, 1>(a, s) : run_attn<T, D, 0, 2>(a, s);
 }
 template <class T> hipError_t run_dim(int D, const pattn_args& a, hipStream_t s) {
     return D == 32 ? run_all<T, 32>(a, s) : D == 64 ? run_all<T, 64>(a, s) : run_all<T, 128>(a, s);
@@ -589,29 +632,50 @@ template <class T> hipError_t run_dim(int D, const pattn_args& a, hipStream_t s)
 
 // Which workgroups take the shared positions, and into how many parts the keys go.
 bool tree_attn_split(int D, pattn_args& a) {
-    const int nto = 16 * attn_col_groups(D, (long long)a.max_rows * a.grp), nts = 16 * attn_col_groups(D, (long long)a.rows * a.grp);
-    const long long cols = (long long)a.rows * a.grp, own = cols / nto + a.n, all = (cols + nts - 1) / nts;
+    const long long cols = (long long)a.rows * a.grp, most = (long long)a.max_rows * a.grp;
+    // Column groups of 16 a workgroup takes. Wide tiles read a block of keys fewer times, narrow ones make more workgroups that run
+    // at once, so the work of all columns decides (columns times positions times kv heads, w), where one group does not hold a
+    // request's columns. us by 1, 2 and 4 groups of heads of 64, 8 kv heads: 64 requests x 8 words over 500 positions (w 4 million) 12.9, 16.5
+    // and 28.9, one of 64 words over 4096 (8) 15.8, 18.2 and 23.2, 8 x 64 over 2500 (23) 23.2, 21.5 and 33.9, one of 33 words over
+    // 32749 (17) 52, 30 and 30; 64 x 32 over 4096 (136) 118, 86 and 92, 64 x 64 over 4096 (273) 222, 147 and 138.
+    // Heads of 128 hold twice the registers, two groups are the most without spills: 1 and 2 of 4 kv heads, 64 x 16 over 4096 98 and 62, 64 x 4
+    // over 4096 (one group holds it) 44.8 and 57
+    a.nts = cols <= 16 ? 1 : 2;
+    auto groups = [&](long long range) {
+        if (a.window) range = std::min(range, a.window + 63ll + a.max_rows);
+        const double w = (double)cols * range * a.n_kv;
+        return most <= 16 || (D <= 64 && w <= 12e6) ? 1 : D > 64 || most <= 32 || w < 200e6 ? 2 : 4;
+    };
+    a.nto = groups(a.prefix_len + a.max_len);
+    long long own = cols / (16 * a.nto) + a.n;
+    const long long all = (cols + 16 * a.nts - 1) / (16 * a.nts);
     auto split = [&](long long tiles, long long range, long long want, int* parts, int* chunk) {
-        const long long p = std::max(std::min(want / std::max(tiles * a.n_kv, 1ll), (range + 255) / 256), 1ll);
+        const long long p = std::max(std::min(want / std::max(tiles * a.n_kv, 1ll), (range + 511) / 512), 1ll);
         *chunk = (int)std::max(((range + p - 1) / p + 127) / 128 * 128, 128ll);
         *parts = (int)std::max((range + *chunk - 1) / *chunk, 1ll);
     };
     a.own_at = (a.prefix_len + 31) / 32 * 32;
     // Requests read the shared positions themselves where their columns fill their workgroups (sharing would save no reads, and
     // nothing has to be joined), and where they are few or the shared positions are: sharing costs a launch and the parts' sums.
-    // us apart and fused, by requests x words behind shared positions, 1000 own ones: 8 kv heads of 64: 64 x 64 behind 1024 151
-    // and 92, 64 x 24 behind 4096 113 and 112; with more than twice as many tiles of requests as of all columns 8 x 4 behind 4096 23 and
-    // 18 (tiles times positions 49152), 64 x 4 behind 1024 35 and 25 (98304), 32 x 2 behind 4096 29 and 33 (163840), 64 x 8
-    // behind 4096 59 and 88 (327680). 4 of 128, whose tiles are half as wide: up to three times as many tiles 32 x 8 behind 1024 32 and 26
-    // (49152), 64 x 8 behind 4096 48 and 58 (393216), above 8 x 4 behind 256 15.7 and 16.5 (3072), behind 1024 16.3 and 18.6
-    a.fused = a.prefix_len == 0 || own <= all * 2 || own * a.prefix_len <= (D <= 64 ? 100000 : own <= all * 3 ? 200000 : 4096);
+    // us apart and fused, by requests x words behind shared positions, 1000 own ones: 8 kv heads of 64: 64 x 64 behind 1024 144
+    // and 85, 64 x 24 behind 4096 105 and 87; with more than twice as many tiles of requests as of all columns 8 x 4 behind 1024 14.2 and
+    // 14.4 (tiles times positions 12288), 64 x 4 behind 1024 28 and 23 (98304), 32 x 2 behind 4096 21 and 31 (163840), 64 x 8
+    // behind 4096 60 and 54 (393216: the rule's loss). 4 of 128: up to three times as many tiles 64 x 8 behind 1024 36 and 33
+    // (98304), behind 4096 50 and 57 (393216), above 2 x 2 behind 256 18.7 and 16.9 (512), 8 x 4 behind 256 15.7 and 17.9 (3072), 32 x 2 behind 256 17 and 28 (10240)
+    a.fused = a.prefix_len == 0 || own <= all * 2 || own * a.prefix_len <= (D <= 64 ? 100000 : own <= all * 3 ? 200000 : 2000);
     a.sp = a.pchunk = 0;
+    if (!a.fused) {
+        a.nto = std::min(groups(a.max_len), 2);
+        own = cols / (16 * a.nto) + a.n;
+    }
     if (!a.fused) split(all, a.window && a.window + 31ll < a.prefix_len ? a.window + 31ll : a.prefix_len, 512, &a.sp, &a.pchunk);
     long long range = (a.fused ? a.own_at : 0ll) + a.max_len;
     if (a.window) range = std::min(range, a.window + 63ll + a.max_rows);
-    // One and a half workgroups per compute unit, of 256 keys or more: one request of up to 32749 positions and 33 words (4 kv heads of
-    // 128) 28 to 29 us, with half as many parts 35, with twice as many 46 (the join reads all of them)
-    split((cols + nto - 1) / nto, range, 384, &a.so, &a.ochunk);
+    // One workgroup per compute unit, of 512 keys or more: one request of 64 words over 33000 positions (8 kv heads of 64) 32 us, with
+    // three quarters as many parts 37, with one and a half times as many 35 (the join reads all of them); 4 kv heads of 128 31, 34 and 36.
+    // 64 requests x 4 words behind 2048 shared positions, 4 kv heads of 128, by 256, 512 and 1024 keys a part 44.8, 39.7 and 38.5,
+    // 8 of 64 35.4, 35.1 and 38.6
+    split(std::max((cols + 16 * a.nto - 1) / (16 * a.nto), (long long)a.n), range, 256, &a.so, &a.ochunk);
     const long long shared_blocks = all * a.n_kv * a.sp, own_blocks = own * a.n_kv * a.so;
     const long long rh = (long long)a.rows * a.n_head, join = a.sp + a.so == 1 ? 0 : a.sp + a.so > 16 ? rh : (rh + 3) / 4;
     // (columns of one kv head are counted in 32 bits in the kernel)
