@@ -81,9 +81,7 @@ template <int NT> __global__ __launch_bounds__(NT) void k_tree_plan(tree_plan_ar
 // and goes on with the first.
 constexpr int PER = TREE_MAX / 64;
 
-__global__ __launch_bounds__(256) void k_tree_take(tree_take_args a) {
-    const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (i >= a.n) return;
+__device__ __forceinline__ void take_branch(const tree_take_args& a, const int i, const int lane) {
     const tree_rows t = rows_of(a.cu, a.held, a.len, i, a.rows, TREE_MAX);
     if (!t.sound || t.m == 0) {
         for (int r = lane; r < t.m; r += 64) a.path[t.r0 + r] = -1;
@@ -135,11 +133,10 @@ __global__ __launch_bounds__(256) void k_tree_take(tree_take_args a) {
     }
 }
 
-// Pages behind the new lengths go back to the list of free ones, in the order of the requests.
+// Pages behind the new lengths go back to the list of free ones, in the order of the requests. One workgroup.
 constexpr int FREE_T = 1024;
 
-__global__ __launch_bounds__(FREE_T) void k_tree_free(tree_take_args a) {
-    __shared__ long long sum_s[FREE_T / 64];
+__device__ __forceinline__ void free_pages_behind(const tree_take_args& a, long long (&sum_s)[FREE_T / 64]) {
     const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
     const int per = (a.n + FREE_T - 1) / FREE_T, i0 = min(a.n, t * per), i1 = min(a.n, i0 + per);
     auto pages = [&](int len) { return (int)min(((long long)max(len, 0) + (1 << a.page_log) - 1) >> a.page_log, (long long)a.cols); };
@@ -165,6 +162,22 @@ __global__ __launch_bounds__(FREE_T) void k_tree_free(tree_take_args a) {
         for (int p = pages(a.len_out[i]), p1 = pages(a.len[i]); p < p1; p++, to++)
             if (to < taken) a.free_pages[to] = a.table[(size_t)i * a.cols + p];
     if (t == 0) a.taken_out[0] = left;
+}
+
+__global__ __launch_bounds__(256) void k_tree_take(tree_take_args a) {
+    const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i < a.n) take_branch(a, i, threadIdx.x & 63);
+}
+__global__ __launch_bounds__(FREE_T) void k_tree_free(tree_take_args a) {
+    __shared__ long long sum_s[FREE_T / 64];
+    free_pages_behind(a, sum_s);
+}
+// both, for requests so few that one workgroup's waves walk them
+__global__ __launch_bounds__(FREE_T) void k_tree_take_free(tree_take_args a) {
+    __shared__ long long sum_s[FREE_T / 64];
+    for (int i = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); i < a.n; i += FREE_T / 64) take_branch(a, i, threadIdx.x & 63);
+    __syncthreads();
+    free_pages_behind(a, sum_s);
 }
 
 // ---------------------------------------------------------------- keys and values of the branch
@@ -234,7 +247,15 @@ hipError_t launch_tree_plan(const tree_plan_args& a, hipStream_t s) {
     return hipGetLastError();
 }
 
+// One launch where a wave walks two requests at most: us by one and two launches, requests of up to 64 words: 2 10.6 and 12.7, 32 10.1
+// and 12.6, 64 12.1 and 12.5 (of up to 256 words 13.8 and 12.0), 128 20.6 and 12.2
+constexpr int FEW = 2 * FREE_T / 64;
+
 hipError_t launch_tree_take(const tree_take_args& a, hipStream_t s) {
+    if (a.table && a.n <= FEW) {
+        k_tree_take_free<<<1, FREE_T, 0, s>>>(a);
+        return hipGetLastError();
+    }
     k_tree_take<<<(a.n + 3) / 4, 256, 0, s>>>(a);
     if (a.table) k_tree_free<<<1, FREE_T, 0, s>>>(a);
     return hipGetLastError();

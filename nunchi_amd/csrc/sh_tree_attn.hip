@@ -14,10 +14,12 @@ namespace {
 constexpr int MASK_WORDS = TREE_MAX / 32;
 
 template <int D, int NT> struct tree_space {
+    static constexpr int PITCH = D + 4;        // (shifts columns by four banks)
     union {
-        join_space<D, NT> join;
-        unsigned short keys[4][32 * (D + 8)];  // each wave's block of keys (the pitch shifts rows by four banks)
-    };
+        float o[16 * NT * PITCH];              // a wave's sums
+        unsigned short keys[32 * (D + 8)];     // its block of keys (the pitch shifts rows by four banks)
+    } wave[4];
+    f32x4 m[16 * NT], l[16 * NT];              // the waves' references and sums of weights
     unsigned mask[16 * NT][MASK_WORDS + 1];    // the columns' masks, and a word without bits
     int lo[16 * NT], hi[16 * NT];              // what a column sees (below)
     float top[4][16 * NT];                     // the largest score of each wave's first block
@@ -96,10 +98,9 @@ __device__ __forceinline__ tile_of_request find_tile(const pattn_args& a, int at
 // shared ones before them where no SHARED part takes them (a.fused).
 template <class T, int D, int NT, bool SHARED>
 __device__ __forceinline__ void attend(const pattn_args& a, const int block, tree_space<D, NT>& s) {
-    constexpr int NC = 16 * NT, E = D / 16, CH = D / 32, VW = E / 2, PITCH = join_space<D, NT>::PITCH;
+    constexpr int NC = 16 * NT, E = D / 16, CH = D / 32, VW = E / 2, PITCH = tree_space<D, NT>::PITCH;
     // f16 weights up to 2^15: their last place is 2^-32 of the largest or less, which a million keys add up to a quarter of half a place
     constexpr float LIFT = mat<T>::LIFT > 0.0f ? 8.0f : 0.0f, SLACK = mat<T>::LIFT > 0.0f ? 7.0f : mat<T>::SLACK;
-    join_space<D, NT>& js = s.join;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m16 = lane & 15, quad = lane >> 4;
     const int S = SHARED ? a.sp : a.so, per = a.n_kv * S;
     // (workgroups of the same keys are `per` apart: on one XCD where that is a multiple of 8)
@@ -134,11 +135,13 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
         for (int w = threadIdx.x % PER; w <= a.words; w += PER) s.mask[c][w] = w < a.words ? from[w] : 0u;
     }
     u32x4 qf[CH][NT];
-#pragma unroll
-    for (int t = 0; t < NT; t++)
+    auto load_queries = [&](int t) {
 #pragma unroll
         for (int c = 0; c < CH; c++)
             qf[c][t] = *(const u32x4*)((const T*)a.q + ((size_t)row_of(16 * t + m16) * a.n_head + head_of(16 * t + m16)) * D + c * 32 + quad * 8);
+    };
+#pragma unroll
+    for (int t = 0; t < NT; t++) load_queries(t);
     __syncthreads();
     // ---- what each column sees: of keys lo .. hi - 1 all before words_at, and the words there whose bits its mask has ----
     const int L0 = a.prefix_len, P = a.own_at;
@@ -244,8 +247,8 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
                 kr[n] = *(const u32x4*)(p + k_lane);
             }
         };
-        unsigned short* const kw = s.keys[wv] + lane / RL * (D + 8) + lane % RL * 8;
-        const unsigned short* const ks = s.keys[wv] + m16 * (D + 8) + quad * 8;
+        unsigned short* const kw = s.wave[wv].keys + lane / RL * (D + 8) + lane % RL * 8;
+        const unsigned short* const ks = s.wave[wv].keys + m16 * (D + 8) + quad * 8;
         auto turn_keys = [&]() {
 #pragma unroll
             for (int n = 0; n < KI; n++) *(u32x4*)(kw + n * RI * (D + 8)) = kr[n];
@@ -334,7 +337,9 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
         // of a lane's eight keys those that its column sees
         auto sees = [&](int t, int kt, int id0, int id1) {
             const bool in_shared = SHARED || kt < P;
-            const int c = 16 * t + m16, from = s.lo[c], stop = min(s.hi[c], in_shared ? L0 : hi1);
+            int self = lane;               // (unknown to the compiler: what follows from it is not kept in registers from block to block)
+            asm volatile("" : "+v"(self));
+            const int c = 16 * t + (self & 15), quad = self >> 4, from = s.lo[c], stop = min(s.hi[c], in_shared ? L0 : hi1);
             unsigned bits = 0;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -422,6 +427,7 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
                 for (int t = 0; t < NT; t++) {
                     bits[t] = sees(t, first + 128 * n, __builtin_amdgcn_readlane(ids0, n), __builtin_amdgcn_readlane(ids1, n));
                     any_sees |= bits[t];
+                    __builtin_amdgcn_sched_barrier(0);
                 }
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
@@ -432,6 +438,7 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
                     const float top = largest(x);
                     if (__any(top > thr[t])) move_to(t, top);
                     weights(t, x);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
                 any_sees = any_of_16(any_sees);
                 unsigned full = 0;             // (a value whose exponent bits are all set carries into its sign)
@@ -453,14 +460,34 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
                             if ((vw[k][w] >> 16 & mat<T>::EXP) == mat<T>::EXP) vw[k][w] &= 0x0000FFFFu;
                         }
                 }
+                __builtin_amdgcn_sched_barrier(0);
                 turn_values();
 #pragma unroll
                 for (int t = 0; t < NT; t++) add_values(t);
+                __builtin_amdgcn_sched_barrier(0);
                 turn_keys();
                 ask_keys(n + 2);
                 ask_values(++n);
                 if (n >= many) break;
                 }
+        }
+        // ---- the wave's sums to LDS, behind the last of its keys ----
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const int c = 16 * t + m16;
+            l[t] += __shfl_xor(l[t], 16);
+            l[t] += __shfl_xor(l[t], 32);
+            if (quad == 0) {
+                ((float*)&s.m[c])[wv] = thr[t] == -INFINITY ? -INFINITY : -nref[t];
+                ((float*)&s.l[c])[wv] = l[t];
+            }
+#pragma unroll
+            for (int k = 0; k < E; k++) {
+                f32x4 x;
+#pragma unroll
+                for (int r = 0; r < 4; r++) x[r] = o[(4 * k + r) % E][t][(4 * k + r) / E];
+                *(f32x4*)(s.wave[wv].o + c * PITCH + quad * 4 * E + 4 * k) = x;
+            }
         }
         if (odd) {
             // Infinities and NaN that some columns of a block see: how many a column sees of either sign (NaN: of both, and so an
@@ -469,13 +496,17 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
             for (kt = k0 + 32 * wv; kt < k1; kt += 128) {
                 const int id0 = id_of(kt, 0), id1 = id_of(kt, 1);
                 if (is_full(kt, id0, id1)) continue;
-                load_keys(half_of(kt, 0, id0), half_of(kt, 1, id1));
-                load_values(half_of(kt, 0, id0), half_of(kt, 1, id1));
-                turn_keys();
+                const unsigned half0 = half_of(kt, 0, id0), half1 = half_of(kt, 1, id1);
+                load_values(half0, half1);
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int c = 0; c < CH; c++) kf[h][c] = *(const u32x4*)((const T*)a.keys + (size_t)(h ? half1 : half0) * (16 * D) + m16 * D + c * 32 + quad * 8);
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     const unsigned bits = sees(t, kt, id0, id1);
                     float x[8];
+                    load_queries(t);
                     scores(t, x);
                     u32x4 st, nt;              // ones for the keys that the column sees, and for those of them without weight
 #pragma unroll
@@ -502,89 +533,68 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
                         const f32x4 less = mat<T>::mul(up, nt, mat<T>::mul(down, st, f32x4{0, 0, 0, 0}));
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
-                            if (plus[r] > 0.0f) o[e][t][r] += INFINITY;
-                            if (less[r] > 0.0f) o[e][t][r] -= INFINITY;
+                            float& at = s.wave[wv].o[(16 * t + m16) * PITCH + quad * 4 * E + r * E + e];
+                            if (plus[r] > 0.0f) at += INFINITY;
+                            if (less[r] > 0.0f) at -= INFINITY;
                         }
                     }
                 }
             }
         }
     }
-    float m[NT];
-#pragma unroll
-    for (int t = 0; t < NT; t++) m[t] = thr[t] == -INFINITY ? -INFINITY : -nref[t];
+    // ---- the four waves joined: their sums through LDS, then each thread adds up four neighbouring dimensions of a column ----
+    constexpr int LD = D / 4, STEP = 256 / LD, TURNS = (NC + STEP - 1) / STEP;   // threads a column, columns at once
     const bool alone = a.sp + a.so == 1;
-    float gate[NT];
+    const int d = threadIdx.x % LD * 4, with = any ? min((k1 - k0 + 31) / 32, 4) : 0;   // (waves from `with` on had no block)
+    float gate[TURNS];
+    if (alone && a.gate) {
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-        const int c = 16 * t + m16;
-        gate[t] = alone && a.gate && wv == 0 ? a.gate[(size_t)row_of(c) * a.n_head + head_of(c)] : INFINITY;
-    }
-    __syncthreads();                       // (their keys' space is the join's)
-    // ---- the four waves joined: 2 and 3 into 0 and 1, then 1 into 0 ----
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-        l[t] += __shfl_xor(l[t], 16);
-        l[t] += __shfl_xor(l[t], 32);
-    }
-#pragma unroll
-    for (int step = 2; step > 0; step >>= 1) {
-        if (k0 + 32 * step >= k1) continue;   // (waves from `step` on had no block)
-        if (wv >= step && wv < 2 * step) {
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const int c = 16 * t + m16;
-                if (quad == 0) {
-                    js.m[wv - step][c] = m[t];
-                    js.l[wv - step][c] = l[t];
-                }
-#pragma unroll
-                for (int e = 0; e < E; e++) *(f32x4*)(js.o[wv - step] + c * PITCH + quad * 4 * E + e * 4) = o[e][t];
-            }
+        for (int n = 0; n < TURNS; n++) {
+            const int c = n * STEP + threadIdx.x / LD;
+            gate[n] = a.gate[(size_t)row_of(c) * a.n_head + head_of(c)];
         }
-        __syncthreads();
-        if (wv < step) {
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const int c = 16 * t + m16;
-                const float m2 = js.m[wv][c], l2 = js.l[wv][c];
-                const float to = fmaxf(m[t], m2), f1 = rescale(m[t], to), f2 = rescale(m2, to);
-                m[t] = to;
-                l[t] = l[t] * f1 + l2 * f2;
-#pragma unroll
-                for (int e = 0; e < E; e++) o[e][t] = o[e][t] * f1 + *(const f32x4*)(js.o[wv] + c * PITCH + quad * 4 * E + e * 4) * f2;
-            }
-        }
-        __syncthreads();
     }
-    if (wv) return;
+    __syncthreads();
+    float top[TURNS], sum[TURNS];
+    f32x4 x[TURNS], f[TURNS];
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-        const int c = 16 * t + m16;
-        if (c0 + c >= ncol) continue;
+    for (int n = 0; n < TURNS; n++) {
+        const int c = min(n * STEP + (int)threadIdx.x / LD, NC - 1);
+        const f32x4 m4 = s.m[c], l4 = s.l[c];
+        top[n] = -INFINITY;
+        sum[n] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; w++)
+            if (w < with) top[n] = fmaxf(top[n], m4[w]);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            f[n][w] = rescale(m4[w], top[n]);
+            if (w < with) sum[n] += l4[w] * f[n][w];
+        }
+        x[n] = f32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        if (w >= with) break;
+#pragma unroll
+        for (int n = 0; n < TURNS; n++) x[n] += *(const f32x4*)(s.wave[w].o + min(n * STEP + (int)threadIdx.x / LD, NC - 1) * PITCH + d) * f[n][w];
+    }
+#pragma unroll
+    for (int n = 0; n < TURNS; n++) {
+        const int c = n * STEP + threadIdx.x / LD;
+        if (c >= NC || c0 + c >= ncol) continue;
         const size_t rh = (size_t)row_of(c) * a.n_head + head_of(c);
         if (alone) {
-            float f = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
-            f *= 1.0f / (1.0f + expf(-gate[t]));       // (no gate: 1)
-            unsigned* dst = (unsigned*)((T*)a.out + rh * D + quad * 4 * E);
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-#pragma unroll
-                for (int e = 0; e < E; e += 2) {
-                    const float x = o[e][t][r], y = o[e + 1][t][r];
-                    dst[(r * E + e) / 2] = l[t] == 0.0f ? 0u : pack2<T>(x * f, y * f);
-                }
-            if (a.lse && quad == 0) a.lse[rh] = l[t] == 0.0f ? -INFINITY : (m[t] + log2f(l[t])) * 0.69314718055994531f;
+            float per = 1.0f / sum[n];
+            if (a.gate) per *= 1.0f / (1.0f + expf(-gate[n]));
+            uint2 y = {0u, 0u};
+            if (sum[n] != 0.0f) y = {pack2<T>(x[n][0] * per, x[n][1] * per), pack2<T>(x[n][2] * per, x[n][3] * per)};
+            *(uint2*)((T*)a.out + rh * D + d) = y;
+            if (a.lse && d == 0) a.lse[rh] = sum[n] == 0.0f ? -INFINITY : (top[n] + log2f(sum[n])) * 0.69314718055994531f;
         } else {
             const size_t at = (size_t)(SHARED ? part : a.sp + part) * a.rows * a.n_head + rh;
-            if (quad == 0) a.part_ml[at] = make_float2(m[t], l[t]);
-            if (any) {
-                float* dst = a.part_o + at * D + quad * 4 * E;
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-#pragma unroll
-                    for (int e = 0; e < E; e++) dst[r * E + e] = o[e][t][r];
-            }
+            if (d == 0) a.part_ml[at] = make_float2(top[n], sum[n]);
+            if (any) *(f32x4*)(a.part_o + at * D + d) = x[n];
         }
     }
 }
