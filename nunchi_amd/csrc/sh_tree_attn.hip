@@ -335,16 +335,20 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
             for (int e = 0; e < E; e++) o[e][t] = mat<T>::mul(vf[e], u32x4{pw[t][0], pw[t][1], pw[t][2], pw[t][3]}, o[e][t]);
         };
         // of a lane's eight keys those that its column sees
-        auto sees = [&](int t, int kt, int id0, int id1) {
-            const bool in_shared = SHARED || kt < P;
-            int self = lane;               // (unknown to the compiler: what follows from it is not kept in registers from block to block)
+        // (the lane's number, unknown to the compiler: what follows from it is not kept in registers from block to block)
+        auto lane_here = [&]() {
+            int self = lane;
             asm volatile("" : "+v"(self));
-            const int c = 16 * t + (self & 15), quad = self >> 4, from = s.lo[c], stop = min(s.hi[c], in_shared ? L0 : hi1);
+            return self;
+        };
+        auto sees = [&](int t, int kt, bool known0, bool known1) {
+            const bool in_shared = SHARED || kt < P;
+            const int self = lane_here(), c = 16 * t + (self & 15), quad = self >> 4, from = s.lo[c], stop = min(s.hi[c], in_shared ? L0 : hi1);
             unsigned bits = 0;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int first = kt + 16 * h + quad * 4;
-                unsigned four = known(h ? id1 : id0) ? 0xFu : 0u;
+                unsigned four = (h ? known1 : known0) ? 0xFu : 0u;
                 if (!SHARED && !in_shared) four &= tree_bits(s.mask[c], a.words, first - words_at);
                 four &= from - first >= 4 ? 0u : 0xFu << max(from - first, 0);
                 bits |= (four & (stop <= first ? 0u : 0xFu >> max(4 - (stop - first), 0))) << (4 * h);
@@ -360,6 +364,7 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
             const int many = min((k1 - first + 127) / 128, 63), lanes = first + 128 * min(lane, many - 1);
             const int ids0 = id_of(lanes, 0), ids1 = id_of(lanes, 1);
             const unsigned long long whole = __ballot(lane < many && is_full(lanes, ids0, ids1));
+            const unsigned long long known0 = __ballot(known(ids0)), known1 = __ballot(known(ids1));
             const unsigned halves0 = half_of(lanes, 0, ids0), halves1 = half_of(lanes, 1, ids1);
             // (behind the last block it is asked for again)
             auto ask_keys = [&](int n) { load_keys(__builtin_amdgcn_readlane(halves0, min(n, many - 1)), __builtin_amdgcn_readlane(halves1, min(n, many - 1))); };
@@ -374,6 +379,7 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
             if (start) {
                 // The first reference is the largest of all four waves' first blocks: far fewer scores pass it by the slack later on
                 start = false;
+                const int self = lane_here(), m16 = self & 15, quad = self >> 4;
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     float x[8];
@@ -425,7 +431,7 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
                 unsigned any_sees = 0, bits[NT];
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    bits[t] = sees(t, first + 128 * n, __builtin_amdgcn_readlane(ids0, n), __builtin_amdgcn_readlane(ids1, n));
+                    bits[t] = sees(t, first + 128 * n, known0 >> n & 1, known1 >> n & 1);
                     any_sees |= bits[t];
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -472,6 +478,7 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
                 }
         }
         // ---- the wave's sums to LDS, behind the last of its keys ----
+        const int self = lane_here(), m16 = self & 15, quad = self >> 4;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             const int c = 16 * t + m16;
@@ -504,7 +511,7 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
                     for (int c = 0; c < CH; c++) kf[h][c] = *(const u32x4*)((const T*)a.keys + (size_t)(h ? half1 : half0) * (16 * D) + m16 * D + c * 32 + quad * 8);
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    const unsigned bits = sees(t, kt, id0, id1);
+                    const unsigned bits = sees(t, kt, known(id0), known(id1));
                     float x[8];
                     load_queries(t);
                     scores(t, x);
@@ -599,10 +606,11 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
     }
 }
 
-// waves per SIMD that the registers are to allow
+// Waves per SIMD that the registers are to allow: the most without spills in the loops (heads of 128, one column group, at three
+// waves 64 requests x 4 words over 2048 positions 50 us, at two 30)
 constexpr int waves_of(int D, int nts, int nto) {
     const int nt = nts > nto ? nts : nto;
-    return nt == 4 || (nt == 2 && D > 64) ? 2 : nt == 2 || D > 64 ? 3 : 4;
+    return nt == 4 || D > 64 ? 2 : nt == 2 ? 3 : 4;
 }
 
 template <class T, int D, int NTS, int NTO>
@@ -644,17 +652,17 @@ template <class T> hipError_t run_dim(int D, const pattn_args& a, hipStream_t s)
 bool tree_attn_split(int D, pattn_args& a) {
     const long long cols = (long long)a.rows * a.grp, most = (long long)a.max_rows * a.grp;
     // Column groups of 16 a workgroup takes. Wide tiles read a block of keys fewer times, narrow ones make more workgroups that run
-    // at once, so the work of all columns decides (columns times positions times kv heads, w), where one group does not hold a
-    // request's columns. us by 1, 2 and 4 groups of heads of 64, 8 kv heads: 64 requests x 8 words over 500 positions (w 4 million) 12.9, 16.5
-    // and 28.9, one of 64 words over 4096 (8) 15.8, 18.2 and 23.2, 8 x 64 over 2500 (23) 23.2, 21.5 and 33.9, one of 33 words over
-    // 32749 (17) 52, 30 and 30; 64 x 32 over 4096 (136) 118, 86 and 92, 64 x 64 over 4096 (273) 222, 147 and 138.
-    // Heads of 128 hold twice the registers, two groups are the most without spills: 1 and 2 of 4 kv heads, 64 x 16 over 4096 98 and 62, 64 x 4
-    // over 4096 (one group holds it) 44.8 and 57
+    // at once, so the work of all columns decides (columns times positions times kv heads, w; heads of 128 twice), where one group does
+    // not hold a request's columns. us by 1, 2 and 4 groups of heads of 64, 8 kv heads: 64 requests x 8 words over 500 positions (w 4
+    // million) 12.9, 16.5 and 28.9, one of 64 words over 4096 (8) 15.8, 18.2 and 23.2, 8 x 64 over 2500 (23) 23.2, 21.5 and 33.9; 64 x
+    // 32 over 4096 (136) 118, 86 and 92, 64 x 64 over 4096 (273) 222, 147 and 138. Four groups of heads of 128 do not fit the registers;
+    // by 1 and 2, 4 kv heads: one of 64 words over 4096 (8) 15.0 and 18.2, one of 32 over 16000 (16) 17.0 and 20.1, 64 x 16 over 500
+    // (8) 22.9 and 21.7, 8 x 64 over 2500 (23) 26.8 and 23.9, 64 x 64 over 4096 (273) 186 and 134
     a.nts = cols <= 16 ? 1 : 2;
     auto groups = [&](long long range) {
         if (a.window) range = std::min(range, a.window + 63ll + a.max_rows);
-        const double w = (double)cols * range * a.n_kv;
-        return most <= 16 || (D <= 64 && w <= 12e6) ? 1 : D > 64 || most <= 32 || w < 200e6 ? 2 : 4;
+        const double w = (double)cols * range * a.n_kv * (D > 64 ? 2 : 1);
+        return most <= 16 || w <= 12e6 ? 1 : D > 64 || most <= 32 || w < 200e6 ? 2 : 4;
     };
     a.nto = groups(a.prefix_len + a.max_len);
     long long own = cols / (16 * a.nto) + a.n;
@@ -667,12 +675,11 @@ bool tree_attn_split(int D, pattn_args& a) {
     a.own_at = (a.prefix_len + 31) / 32 * 32;
     // Requests read the shared positions themselves where their columns fill their workgroups (sharing would save no reads, and
     // nothing has to be joined), and where they are few or the shared positions are: sharing costs a launch and the parts' sums.
-    // us apart and fused, by requests x words behind shared positions, 1000 own ones: 8 kv heads of 64: 64 x 64 behind 1024 144
-    // and 85, 64 x 24 behind 4096 105 and 87; with more than twice as many tiles of requests as of all columns 8 x 4 behind 1024 14.2 and
-    // 14.4 (tiles times positions 12288), 64 x 4 behind 1024 28 and 23 (98304), 32 x 2 behind 4096 21 and 31 (163840), 64 x 8
-    // behind 4096 60 and 54 (393216: the rule's loss). 4 of 128: up to three times as many tiles 64 x 8 behind 1024 36 and 33
-    // (98304), behind 4096 50 and 57 (393216), above 2 x 2 behind 256 18.7 and 16.9 (512), 8 x 4 behind 256 15.7 and 17.9 (3072), 32 x 2 behind 256 17 and 28 (10240)
-    a.fused = a.prefix_len == 0 || own <= all * 2 || own * a.prefix_len <= (D <= 64 ? 100000 : own <= all * 3 ? 200000 : 2000);
+    // us apart and fused, by requests x words behind shared positions, 1000 own ones, 8 kv heads of 64, then 4 of 128: 64 x 64 behind
+    // 1024 142 and 85, 114 and 76; 64 x 24 behind 4096 104 and 87, 95 and 89; with more than twice as many tiles of requests as of all
+    // columns 32 x 2 behind 1024 (tiles times positions 40960) 17 and 14, 21 and 19, 64 x 4 behind 1024 (98304) 27 and 23, 27 and 26,
+    // 32 x 2 behind 4096 (163840) 21 and 31, 24 and 30, 64 x 4 behind 4096 (393216) 34 and 48, 40 and 48
+    a.fused = a.prefix_len == 0 || own <= all * 2 || own * a.prefix_len <= 100000;
     a.sp = a.pchunk = 0;
     if (!a.fused) {
         a.nto = std::min(groups(a.max_len), 2);
