@@ -20,7 +20,10 @@ namespace sh {
 namespace {
 
 constexpr int PT = 256;                    // threads of a part
-constexpr int LISTED = 1024;               // words that may be listed
+constexpr int LISTED = 1024;               // words of a part that may be listed
+constexpr int GROUPS = 256, PAST = 4;      // groups of words; how many more than asked for a cut may leave
+// keys that a row's parts may have, and those of them that a cut of their groups can leave at most
+constexpr int JOINED = SAMPLE_MAX_VOCAB / (32 * PT) * PROBS_MAX_TOP, LEFT = ((PROBS_MAX_TOP + PAST) * (JOINED / GROUPS) + 63) / 64 * 64;
 
 template <class T> struct score_vec {
     static constexpr int V = 8;
@@ -71,24 +74,26 @@ template <class K, int N> __device__ __forceinline__ K reached_by(const K (&key)
 #pragma unroll
         for (int e = 0; e < N; e++) c += __popcll(__ballot(key[e] >= (at | bit)));
         if (c >= n) at |= bit;
-        if (c >= n && c <= n + 4) break;
+        if (c >= n && c <= n + PAST) break;
     }
     return at;
 }
 
-// The want largest of n keys in LDS, in order, to best[0 .. want); 0 behind them. One wave.
-__device__ __forceinline__ void order_keys(const u64* key, int n, int want, u64* best, int lane) {
-    if (n <= 64) {                         // one a lane, told to all lanes one after the other
-        const u64 mine = lane < n ? key[lane] : 0;
-        const int hi = (int)(mine >> 32), lo = (int)(unsigned)mine;
-        int before = 0;
-        for (int o = 0; o < n; o++) {
-            const u64 x = (u64)(unsigned)__builtin_amdgcn_readlane(hi, o) << 32 | (unsigned)__builtin_amdgcn_readlane(lo, o);
-            before += x > mine;
+// The want largest of n keys in LDS, in order, to best[0 .. want); 0 behind them. By NT threads: t is one's number among them.
+template <int NT> __device__ __forceinline__ void order_keys(const u64* key, int n, int want, u64* best, int t) {
+    if (n <= 64) {                         // one a lane of the first wave, told to all lanes one after the other
+        if (t < 64) {
+            const u64 mine = t < n ? key[t] : 0;
+            const int hi = (int)(mine >> 32), lo = (int)(unsigned)mine;
+            int before = 0;
+            for (int o = 0; o < n; o++) {
+                const u64 x = (u64)(unsigned)__builtin_amdgcn_readlane(hi, o) << 32 | (unsigned)__builtin_amdgcn_readlane(lo, o);
+                before += x > mine;
+            }
+            if (t < n && before < want) best[before] = mine;
         }
-        if (lane < n && before < want) best[before] = mine;
     } else {
-        for (int k = lane; k < n; k += 64) {
+        for (int k = t; k < n; k += NT) {
             const u64 mine = key[k];
             int before = 0;
 #pragma unroll 8
@@ -96,7 +101,7 @@ __device__ __forceinline__ void order_keys(const u64* key, int n, int want, u64*
             if (before < want) best[before] = mine;
         }
     }
-    for (int k = n + lane; k < want; k += 64) best[k] = 0;
+    for (int k = n + t; k < want; k += NT) best[k] = 0;
 }
 
 // two parts' sums as one, relative to the larger of their largest (c: powers of two a unit of score)
@@ -123,7 +128,7 @@ __device__ __forceinline__ probs_part joined(const probs_part& a, const probs_pa
 __device__ __forceinline__ float per_score(float temp) { return temp > 0.0f ? fminf(1.44269504f / temp, 3e38f) : 1.0f; }
 
 struct join_shared {
-    u64 key[LISTED], best[PROBS_MAX_TOP];
+    u64 key[LEFT > LISTED ? LEFT : LISTED], best[PROBS_MAX_TOP];
     float log_sum, top;
 };
 
@@ -133,33 +138,42 @@ template <class T, int NT> __device__ __forceinline__ void join_row(const probs_
     const float temp = a.temp ? a.temp[row] : 1.0f;
     const int want = a.n_top > 0 ? a.n_top : 1;
     if (wv == 0) {
-        // The want-th largest of the lanes' largest keys: the few from there up hold them all
+        // The keys in groups, four a lane: the want-th largest of the groups' largest, and the few dozen from there up hold them all. (A part's
+        // keys are in order, so a group is to take few keys of each part.)
         const u64* best = a.best + (size_t)row * a.parts * want;
         const int all = a.parts * want;
-        u64 most = 0;
-#pragma unroll 4
-        for (int k = lane; k < all; k += 64) most = max(most, best[k]);
-        const u64 mosts[1] = {most}, cut = max(reached_by(mosts, want), 1ull);
+        u64 most[4] = {0, 0, 0, 0};
+        for (int k = lane; k < all; k += GROUPS) {
+            u64 x[4];
+#pragma unroll
+            for (int g = 0; g < 4; g++) x[g] = k + 64 * g < all ? best[k + 64 * g] : 0;
+#pragma unroll
+            for (int g = 0; g < 4; g++) most[g] = max(most[g], x[g]);
+        }
+        const u64 cut = max(reached_by(most, want), 1ull);
         int n = 0;
 #pragma unroll 4
         for (int k = 0; k < all; k += 64) {
             const u64 mine = k + lane < all ? best[k + lane] : 0;
             const u64 who = __ballot(mine >= cut);
             const int at = n + __popcll(who & ((1ull << lane) - 1));
-            if (mine >= cut && at < LISTED) s.key[at] = mine;
+            if (mine >= cut && at < LEFT) s.key[at] = mine;
             n += __popcll(who);
         }
-        if (n <= LISTED) {
-            order_keys(s.key, n, want, s.best, lane);
-        } else {                           // (hundreds of parts of which a few lanes hold most of the likeliest)
-            for (int k = lane; k < all; k += 64) {
-                const u64 mine = best[k];
-                if (mine < cut) continue;
-                int before = 0;
-                for (int o = 0; o < all && before < want; o++) before += best[o] > mine;
-                if (before < want) s.best[before] = mine;
+        if (n > 128) {                     // (many parts and many words: once more, among the keys themselves)
+            u64 mine[LEFT / 64];
+#pragma unroll
+            for (int e = 0; e < LEFT / 64; e++) mine[e] = 64 * e + lane < n ? s.key[64 * e + lane] : 0;
+            const u64 from = reached_by(mine, want);
+            n = 0;
+#pragma unroll
+            for (int e = 0; e < LEFT / 64; e++) {
+                const u64 who = __ballot(mine[e] >= from);
+                if (mine[e] >= from) s.key[n + __popcll(who & ((1ull << lane) - 1))] = mine[e];
+                n += __popcll(who);
             }
         }
+        order_keys<64>(s.key, n, want, s.best, lane);
     } else if (wv == 1) {
         const probs_part* p = a.part + (size_t)row * a.parts;
         const float c = per_score(temp);
@@ -271,19 +285,13 @@ template <class T, int VPT> __global__ __launch_bounds__(PT) void k_probs_part(p
     if (lane == 0) part_s[wv] = probs_part{top, top == -INFINITY ? 0.0f : (float)ties, rest_w, dist_w};
     if (t == 0) n_s = 0;
     __syncthreads();
-    // ---- where the likeliest begin: groups of four threads' words, or of one's where more than 32 are asked for ----
+    // ---- where the likeliest begin: a group is a thread's words ----
     const int want = a.n_top > 0 ? a.n_top : 1;
     if (wv == 0) {
         unsigned k[4];
 #pragma unroll
         for (int w = 0; w < WAVES; w++) k[w] = lane_s[64 * w + lane];
-        unsigned cut;
-        if (want <= 32) {
-            const unsigned all[1] = {max(max(k[0], k[1]), max(k[2], k[3]))};
-            cut = reached_by(all, want);
-        } else {
-            cut = reached_by(k, want);
-        }
+        const unsigned cut = reached_by(k, want);
         if (lane == 0) cut_s = max(cut, NONE + 1);
     } else if (t == 64) {
         probs_part p = part_s[0];
@@ -326,7 +334,7 @@ template <class T, int VPT> __global__ __launch_bounds__(PT) void k_probs_part(p
         __syncthreads();
         n = min(n_s, LISTED);
     }
-    if (wv == 0) order_keys(key_s, n, want, a.best + ((size_t)row * a.parts + part) * want, lane);
+    order_keys<PT>(key_s, n, want, a.best + ((size_t)row * a.parts + part) * want, t);
     if (a.parts == 1) {
         __syncthreads();
         join_row<T, PT>(a, row, js);
@@ -352,11 +360,11 @@ template <class T> hipError_t run_probs(const probs_args& a, hipStream_t s) {
 
 }  // namespace
 
-// One part where 8192 words hold the row, so that one launch is all. Else parts of 8192 words, or of 2048 where the rows are too
-// few to fill the compute units with those.
+// Parts of 8192 words, 32 a thread: as many as the registers hold, so that a row of up to 8192 words is one part and one launch is all
+// (8000 words: 10.2 us, in parts of 2048 12.4). us by parts of 2048 and 8192, rows of f32 scores: 256 of 97496 35 and 26, one with its
+// 5 likeliest words 12.3 and 11.9, with 20 14.6 and 12.7, with 64 32.6 and 22.7. 2048 words are one part of 8 a thread.
 void word_probs_split(probs_args& a) {
-    const int large = 32 * PT, small = 8 * PT;
-    a.chunk = a.vocab <= small ? small : a.vocab <= large || (long long)a.rows * ((a.vocab + large - 1) / large) >= 512 ? large : small;
+    a.chunk = a.vocab <= 8 * PT ? 8 * PT : 32 * PT;
     a.parts = (a.vocab + a.chunk - 1) / a.chunk;
 }
 
