@@ -89,7 +89,7 @@ def build_module(verbose: bool = False) -> None:
     missing = f"the compiler {cxx}" if not shutil.which(cxx) else "Python.h" if not os.path.exists(os.path.join(include, "Python.h")) else None
     if missing:
         drop(untagged, MODULE)
-        sys.stderr.write(f"{missing} is not there: {os.path.basename(MODULE)} (page_plan, page_put, page_attn and sample from Python) is not built\n")
+        sys.stderr.write(f"{missing} is not there: {os.path.basename(MODULE)} (the batch operators, page_plan to page_keep, from Python) is not built\n")
         return
     tmp = MODULE + f".tmp{os.getpid()}"
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-I", include, "-o", tmp, os.path.join(HERE, "csrc", "py_batch.cpp")]

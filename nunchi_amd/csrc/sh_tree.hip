@@ -1,5 +1,8 @@
 // Trees of drafted words: their masks and positions (k_tree_plan), the branch that the picked words agree with (k_tree_take)
 // and the pages that are free again after it (k_tree_free), and the branch's keys and values at their places (k_page_keep).
+//
+// All are bound by latency: 256 requests of 64 words read and write 1 MB (plan), 0.3 MB (take), 16 MB (keep, of up to 15 moved
+// words); a launch with its dependent loads takes 3 to 6 us, and the calling thread 8 to 10 us for each call that it makes.
 #include <hip/hip_runtime.h>
 
 #include <climits>
@@ -241,6 +244,8 @@ template <int D> __global__ __launch_bounds__(256) void k_page_keep(keep_args a)
 
 }  // namespace
 
+// A wave a request where it holds the largest tree, so that a turn waits for no other wave: us by 64 and 256 threads, trees of 64 words,
+// 256 requests 8.5 and 8.7, 4096 8.0 and 12.3
 hipError_t launch_tree_plan(const tree_plan_args& a, hipStream_t s) {
     if (a.max_rows <= 64) k_tree_plan<64><<<a.n, 64, 0, s>>>(a);
     else k_tree_plan<TREE_MAX><<<a.n, TREE_MAX, 0, s>>>(a);

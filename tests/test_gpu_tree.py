@@ -490,6 +490,14 @@ def test_probs_largest_vocab(ctx):
         check_probs(ctx, scores, None, words, 64)
 
 
+@pytest.mark.parametrize("top", [1, 20, 63, 64])
+def test_probs_likeliest_words_of_many_parts(ctx, top):
+    """The likeliest words spread evenly over the largest row, in every part's first places, and in steps from part to part."""
+    i = np.arange(524288)
+    x = np.stack([-(i % 8192.0), -(i % 8192) + (i // 8192) * 0.25, -(i % 8192) - (i // 8192) * 16.0, np.cos(i * 0.7)])
+    check_probs(ctx, dev(x.astype(np.float32)), None, None, top)
+
+
 @pytest.mark.parametrize("spread,temp", [(0.0, 1.0), (0.01, 1.0), (30.0, 1.0), (1000.0, 0.5), (1e30, 1e30), (1e-20, 1e-21), (3.0, 1e-38), (3.0, math.inf), (1e38, 1.0)])
 def test_probs_scales(ctx, spread, temp):
     """From all words alike to one that has everything, and temperatures at the ends of the range."""
