@@ -6,7 +6,7 @@
 // r' = max(r1, r2), l' = l1 e^(r1 - r') + l2 e^(r2 - r'), O' likewise, and the result is O / l (0 where nothing is seen).
 //
 // What bounds it: many columns, issue: 64 requests of up to 64 words over 2048 shared and 2048 own positions (8 kv heads of 64, 56
-// GFLOP) 120 to 131 us, 430 to 470 TFLOP/s of 1139, of which the exponentials, conversions and masks take as long as the products,
+// GFLOP) 120 to 133 us, 420 to 470 TFLOP/s of 1139, of which the exponentials, conversions and masks take as long as the products,
 // and 2.1 rounds of workgroups over the compute units; few columns over long keys, memory: 64 requests x 4 words behind 2048 shared
 // and 2048 own positions 35 us, 4.8 TB/s of 5.0; one request, the chain of loads in front of the first product (ids, keys, 5 us) and
 // the join of its parts (6 us of 22 to 29 for 32749 positions); short ones, the launch.
