@@ -464,8 +464,9 @@ int sh_word_probs(sh_ctx* ctx, int rows, int vocab, const void* scores, long lon
  *   count   [n]     kept rows
  *   next    [n]     the pick after the last kept row: the word that the next step starts with (-1 where there is none)
  *   len_out [n]     held + count
- * Picks below 0 agree with nothing. A request without rows keeps its length; one that was refused (as above) keeps nothing, its
- * len_out is len. With table [n][cols] (null: not done) the pages between ceil(len_out / page) and ceil(len / page) of each
+ * Picks below 0 agree with nothing. A request without rows keeps its length; one whose length is not held + its rows, or that has
+ * more than 256 rows, keeps nothing, its len_out is len. One whose first row has a parent that is not -1 keeps nothing either, its
+ * len_out is held: none of its rows were written. With table [n][cols] (null: not done) the pages between ceil(len_out / page) and ceil(len / page) of each
  * request go back, in the order of the requests: *taken of free_pages [n_free] were given out (sh_page_plan's taken_out),
  * *taken_out is that less the pages that go back, which are written from free_pages[*taken_out] on; pages past *taken are not
  * written. n up to 4096. */

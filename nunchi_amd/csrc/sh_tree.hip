@@ -86,12 +86,14 @@ constexpr int PER = TREE_MAX / 64;
 
 __device__ __forceinline__ void take_branch(const tree_take_args& a, const int i, const int lane) {
     const tree_rows t = rows_of(a.cu, a.held, a.len, i, a.rows, TREE_MAX);
-    if (!t.sound || t.m == 0) {
+    // (a first row that has a parent among the rows, or none that there is, has no bits: nothing was written for it or behind it)
+    const bool whole = t.sound && t.m > 0, rooted = whole && a.parent[t.r0] == -1;
+    if (!rooted) {
         for (int r = lane; r < t.m; r += 64) a.path[t.r0 + r] = -1;
         if (lane == 0) {
             a.count[i] = 0;
             a.next[i] = -1;
-            a.len_out[i] = a.len[i];
+            a.len_out[i] = whole ? a.held[i] : a.len[i];
         }
         return;
     }
