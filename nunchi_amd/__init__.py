@@ -32,7 +32,8 @@ EXPORTS = [
     "sh_ears_load", "sh_ears_free", "sh_ears_info", "sh_ears_positions", "sh_ears_encode", "sh_ears_mel",
     "sh_bench_empty", "sh_bench_read", "sh_bench_xcc", "sh_bench_l2_reuse",
     "sh_page_plan", "sh_page_put", "sh_page_attn_work", "sh_page_attn", "sh_sample_work", "sh_sample",
-    "sh_tree_plan", "sh_tree_attn_work", "sh_tree_attn", "sh_word_probs_work", "sh_word_probs", "sh_tree_take", "sh_page_keep",
+    "sh_tree_plan", "sh_tree_attn_work", "sh_tree_attn", "sh_word_probs_work", "sh_word_probs", "sh_tree_take",
+    "sh_tree_take_planned", "sh_page_keep",
 ]
 
 
@@ -168,6 +169,7 @@ def load_library(path: str = LIB_PATH):
         "sh_word_probs_work": (i, [i, i, i, P(C.c_size_t)]),
         "sh_word_probs": (i, [vp, i, i, vp, C.c_longlong, i, vp, vp, i, vp, vp, vp, vp, i, vp, C.c_size_t]),
         "sh_tree_take": (i, [vp, i, i, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i, vp, i, vp, i, vp, vp]),
+        "sh_tree_take_planned": (i, [vp, i, i, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i, vp, i, vp, i, vp, vp]),
         "sh_page_keep": (i, [vp, vp, i, i, vp, vp, vp, vp, i, vp, vp]),
     }
     for name, (res, args) in sig.items():

@@ -15,7 +15,7 @@ import ctypes as C
 import nunchi_amd as _n
 
 _TYPES = {"f16": 1, "bf16": 30}
-_ENTRIES = ("sh_page_plan", "sh_page_put", "sh_page_attn", "sh_sample", "sh_tree_plan", "sh_tree_attn", "sh_word_probs", "sh_tree_take", "sh_page_keep")
+_ENTRIES = ("sh_page_plan", "sh_page_put", "sh_page_attn", "sh_sample", "sh_tree_plan", "sh_tree_attn", "sh_word_probs", "sh_tree_take_planned", "sh_page_keep")
 _native = None      # (the module, addresses of _ENTRIES): made by the first call
 
 
@@ -150,13 +150,14 @@ def word_probs(ctx, scores, work, temp=None, words=None, logp=None, entropy=None
 
 
 def tree_take(ctx, cu, parent, words, picks, held, length, path, count, next, length_out, table=None, page: int = 16, free=None, taken=None,
-              taken_out=None):
+              taken_out=None, pos=None):
     """The branch of drafted words that the picks agree with (sh_tree_take): cu [n + 1], parent, words and picks [rows], held
     and length [n] i32 in; path [rows], count, next and length_out [n] i32 out. With table [n][cols] i32 the pages behind the
-    new lengths go back to free [n_free] i32, taken [1] i32 in and taken_out [1] out."""
+    new lengths go back to free [n_free] i32, taken [1] i32 in and taken_out [1] out. With pos [rows] i32, tree_plan's, requests
+    that it refused keep nothing and the length they had (sh_tree_take_planned)."""
     native = _native or _load()
     rc = native[0].tree_take(native[8], ctx.h.value, ctx.device, cu, parent, words, picks, held, length, path, count, next, length_out, table, page, free,
-                             taken, taken_out)
+                             taken, taken_out, pos)
     if rc:
         _n._check(rc)
 

@@ -339,27 +339,28 @@ PyObject* word_probs(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 }
 
 PyObject* tree_take(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-    decltype(&sh_tree_take) fn;
+    decltype(&sh_tree_take_planned) fn;
     sh_ctx* ctx;
     long dev;
-    if (!head(a, n_args, 18, fn, ctx, dev)) return nullptr;
-    tensor cu, parent, words, picks, held, length, path, count, next, length_out, table, free_pages, taken, taken_out;
+    if (!head(a, n_args, 19, fn, ctx, dev)) return nullptr;
+    tensor cu, parent, pos, words, picks, held, length, path, count, next, length_out, table, free_pages, taken, taken_out;
     long long page;
     if (!read(a[3], "cu", dev, K_I32, cu) || !read(a[4], "parent", dev, K_I32, parent) || !read(a[5], "words", dev, K_I32, words) ||
         !read(a[6], "picks", dev, K_I32, picks) || !read(a[7], "held", dev, K_I32, held) || !read(a[8], "length", dev, K_I32, length) ||
         !read(a[9], "path", dev, K_I32, path) || !read(a[10], "count", dev, K_I32, count) || !read(a[11], "next", dev, K_I32, next) ||
         !read(a[12], "length_out", dev, K_I32, length_out) || !read(a[13], "table", dev, K_I32, table) || !number(a[14], I32_MIN, I32_MAX, "page", page) ||
-        !read(a[15], "free", dev, K_I32, free_pages) || !read(a[16], "taken", dev, K_I32, taken) || !read(a[17], "taken_out", dev, K_I32, taken_out))
+        !read(a[15], "free", dev, K_I32, free_pages) || !read(a[16], "taken", dev, K_I32, taken) || !read(a[17], "taken_out", dev, K_I32, taken_out) ||
+        !read(a[18], "pos", dev, K_I32, pos))
         return nullptr;
     if (!packed(cu, parent, "parent")) return nullptr;
     const long long n = cu.d[0] - 1, rows = parent.d[0];
     if (!has(words, "words", 1, rows) || !has(picks, "picks", 1, rows) || !has(held, "held", 1, n) || !has(length, "length", 1, n) || !has(path, "path", 1, rows) ||
-        !has(count, "count", 1, n) || !has(next, "next", 1, n) || !has(length_out, "length_out", 1, n))
+        !has(count, "count", 1, n) || !has(next, "next", 1, n) || !has(length_out, "length_out", 1, n) || !has(pos, "pos", 1, rows, 0, 0, 0, true))
         return nullptr;
     if (!table.none() && (!dims(table, "table", 2) || !fits(table, "table") || !has(table, "table", 2, n, table.d[1]) || !dims(free_pages, "free", 1) ||
                           !fits(free_pages, "free") || !has(taken, "taken", 1, 1) || !has(taken_out, "taken_out", 1, 1)))
         return nullptr;
-    return PyLong_FromLong(fn(ctx, (int)n, (int)rows, (const int32_t*)cu.p, (const int32_t*)parent.p, (const int32_t*)words.p, (const int32_t*)picks.p,
+    return PyLong_FromLong(fn(ctx, (int)n, (int)rows, (const int32_t*)cu.p, (const int32_t*)parent.p, (const int32_t*)pos.p, (const int32_t*)words.p, (const int32_t*)picks.p,
                               (const int32_t*)held.p, (const int32_t*)length.p, (int32_t*)path.p, (int32_t*)count.p, (int32_t*)next.p, (int32_t*)length_out.p,
                               (int)page, (const int32_t*)table.p, (int)table.d[1], (int32_t*)free_pages.p, (int)free_pages.d[0], (const int32_t*)taken.p,
                               (int32_t*)taken_out.p));

@@ -78,7 +78,7 @@ struct tree_plan_args {
 
 struct tree_take_args {
     int n, rows;
-    const int32_t *cu, *parent, *word, *pick, *held, *len;
+    const int32_t *cu, *parent, *pos, *word, *pick, *held, *len;   // (pos: null where it is not asked)
     int32_t *path, *count, *next, *len_out;
     // pages that are free again; none where table is null
     int page_log, cols, n_free;

@@ -468,11 +468,10 @@ int sh_word_probs(sh_ctx* c, int rows, int vocab, const void* scores, long long 
     SH_ENTRY_END
 }
 
-int sh_tree_take(sh_ctx* c, int n, int rows, const int32_t* cu, const int32_t* parent, const int32_t* words, const int32_t* picks, const int32_t* held,
-                 const int32_t* len, int32_t* path, int32_t* count, int32_t* next, int32_t* len_out, int page, const int32_t* table, int cols,
-                 int32_t* free_pages, int n_free, const int32_t* taken, int32_t* taken_out) {
+static int take(const char* who, sh_ctx* c, int n, int rows, const int32_t* cu, const int32_t* parent, const int32_t* pos, const int32_t* words, const int32_t* picks,
+                const int32_t* held, const int32_t* len, int32_t* path, int32_t* count, int32_t* next, int32_t* len_out, int page, const int32_t* table, int cols,
+                int32_t* free_pages, int n_free, const int32_t* taken, int32_t* taken_out) {
     SH_ENTRY
-    const char* who = "sh_tree_take";
     if (!c || n < 1 || rows < 0) return bad(who, "null context, n below 1, or rows negative");
     if (n > PLAN_MAX_N) return bad(who, "n must be 1 to 4096");
     if (!cu || !held || !len || !count || !next || !len_out || (rows && (!parent || !words || !picks || !path))) return bad(who, "null");
@@ -482,7 +481,7 @@ int sh_tree_take(sh_ctx* c, int n, int rows, const int32_t* cu, const int32_t* p
         if (!taken || !taken_out || (n_free && !free_pages)) return bad(who, "null");
     }
     const size_t each = (size_t)n * 4, row4 = (size_t)rows * 4;
-    const extent in[] = {{cu, each + 4}, {parent, row4}, {words, row4}, {picks, row4}, {held, each}, {len, each}, {table, table ? each * cols : 0},
+    const extent in[] = {{cu, each + 4}, {parent, row4}, {pos, row4}, {words, row4}, {picks, row4}, {held, each}, {len, each}, {table, table ? each * cols : 0},
                          {table ? taken : nullptr, 4}},
                  out[] = {{path, row4}, {count, each}, {next, each}, {len_out, each}, {table ? free_pages : nullptr, (size_t)(table ? n_free : 0) * 4},
                           {table ? taken_out : nullptr, 4}};
@@ -494,6 +493,7 @@ int sh_tree_take(sh_ctx* c, int n, int rows, const int32_t* cu, const int32_t* p
     a.rows = rows;
     a.cu = cu;
     a.parent = parent;
+    a.pos = pos;
     a.word = words;
     a.pick = picks;
     a.held = held;
@@ -513,6 +513,20 @@ int sh_tree_take(sh_ctx* c, int n, int rows, const int32_t* cu, const int32_t* p
     }
     return done(launch_tree_take(a, c->stream), who);
     SH_ENTRY_END
+}
+
+int sh_tree_take(sh_ctx* c, int n, int rows, const int32_t* cu, const int32_t* parent, const int32_t* words, const int32_t* picks, const int32_t* held,
+                 const int32_t* len, int32_t* path, int32_t* count, int32_t* next, int32_t* len_out, int page, const int32_t* table, int cols,
+                 int32_t* free_pages, int n_free, const int32_t* taken, int32_t* taken_out) {
+    return take("sh_tree_take", c, n, rows, cu, parent, nullptr, words, picks, held, len, path, count, next, len_out, page, table, cols, free_pages, n_free, taken,
+                taken_out);
+}
+
+int sh_tree_take_planned(sh_ctx* c, int n, int rows, const int32_t* cu, const int32_t* parent, const int32_t* pos, const int32_t* words, const int32_t* picks,
+                         const int32_t* held, const int32_t* len, int32_t* path, int32_t* count, int32_t* next, int32_t* len_out, int page, const int32_t* table,
+                         int cols, int32_t* free_pages, int n_free, const int32_t* taken, int32_t* taken_out) {
+    return take("sh_tree_take_planned", c, n, rows, cu, parent, pos, words, picks, held, len, path, count, next, len_out, page, table, cols, free_pages, n_free, taken,
+                taken_out);
 }
 
 int sh_page_keep(sh_ctx* c, const sh_page_shape* s, int n, int rows, const int32_t* cu, const int32_t* path, const int32_t* len, const int32_t* table,

@@ -85,10 +85,11 @@ template <int NT> __global__ __launch_bounds__(NT) void k_tree_plan(tree_plan_ar
 constexpr int PER = TREE_MAX / 64;
 
 __device__ __forceinline__ void take_branch(const tree_take_args& a, const int i, const int lane) {
-    const tree_rows t = rows_of(a.cu, a.held, a.len, i, a.rows, TREE_MAX);
-    // (a first row that has a parent among the rows, or none that there is, has no bits: nothing was written for it or behind it)
-    const bool whole = t.sound && t.m > 0, rooted = whole && a.parent[t.r0] == -1;
-    if (!rooted) {
+    const tree_rows t = rows_of(a.cu, a.held, a.len, i, a.rows, a.pos ? INT_MAX : TREE_MAX);
+    // Nothing was written for a first row without a position, nor behind it: the plan refused the request, or the row has a parent among
+    // the rows, or none that there is
+    const bool whole = t.sound && t.m > 0, planned = whole && a.parent[t.r0] == -1 && (!a.pos || a.pos[t.r0] >= 0) && t.m <= TREE_MAX;
+    if (!planned) {
         for (int r = lane; r < t.m; r += 64) a.path[t.r0 + r] = -1;
         if (lane == 0) {
             a.count[i] = 0;

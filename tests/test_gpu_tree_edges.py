@@ -38,3 +38,68 @@ def test_take_first_rows_with_a_parent(ctx):
         back = sum((table[i, -(-int(got["length"][i]) // 16):-(-length[i] // 16)].tolist() for i in range(5)), [])
         assert [int(x) for x in table[1, 2:4]] == [x for x in back if x in table[1]] and [int(table[2, 1])] == [x for x in back if x in table[2]]
         assert got["taken"].tolist() == [40 - len(back)] and got["free"][40 - len(back):40].tolist() == back
+
+
+class Planned(tt.Drafting):
+    """Conversations whose steps tell tree_take what tree_plan refused: those of more rows than the step's max_rows."""
+
+    def buffers(self, sizes, max_rows):
+        b = super().buffers(sizes)
+        b.update(max_rows=max_rows, mask=torch.zeros(sum(sizes), (max_rows + 31) // 32, dtype=torch.int32, device="cuda"))
+        return b
+
+    def enqueue(self, b, ctx=None):
+        take = nunchi_amd.tree_take
+        try:
+            nunchi_amd.tree_take = lambda *args, **kw: take(*args, **kw, pos=b["pos"])
+            super().enqueue(b, ctx)
+        finally:
+            nunchi_amd.tree_take = take
+
+    def check(self, b):
+        sizes = [m if m <= b["max_rows"] else 0 for m in b["sizes"]]
+        kept = np.repeat([m > 0 for m in sizes], b["sizes"])
+        rows = torch.from_numpy(np.flatnonzero(kept)).cuda()
+        self.parent, self.words = ([x for x, k in zip(y, kept) if k] for y in (self.parent, self.words))
+        super().check({**b, "sizes": sizes, **{k: b[k][rows] for k in ("out", "scores", "picks", "logp", "entropy", "top", "path")}})
+        assert (b["path"].cpu()[torch.from_numpy(~kept)] == -1).all() and (b["pos"].cpu()[torch.from_numpy(~kept)] == -1).all()
+
+
+@pytest.mark.parametrize("many", [33, 70, 100])
+def test_step_with_a_request_that_the_plan_refused(many):
+    """One conversation drafts more words than the step's max_rows: page_plan gives it pages, tree_plan no bits. It keeps its length, its
+    pages go back, and its next step reads what it held."""
+    s = Planned(nunchi_amd.Context(0, stream=torch.cuda.current_stream().cuda_stream))
+    for sizes, max_rows in [([4, 5, 3, 9], 9), ([9, many, 3, 5], 32), ([5, 8, 1, 3], 8), ([many, many, many, many], many - 1), ([2, 6, 7, 8], 64)]:
+        b = s.buffers(sizes, max_rows)
+        s.draft(b)
+        before = [len(x) for x in s.said]
+        s.enqueue(b)
+        torch.cuda.synchronize()
+        s.check(b)
+        assert [len(x) == k for x, k in zip(s.said, before)] == [m > max_rows for m in sizes]
+        s.check_cache()
+
+
+@pytest.mark.parametrize("page", [16, 64])
+def test_take_requests_that_the_plan_refused(ctx, page):
+    """Those of more rows than max_rows (and than 256) keep nothing and the length before the step; their pages go back."""
+    sizes, max_rows = [5, 40, 257, 0, 40, 39, 300, 2] * 9, 39
+    parent, words, picks, held = tt.take_case(11, sizes, 2)
+    length = held + sizes
+    length[3], held[7] = length[3] - 1, -1       # (refused by the page plan: the length stays)
+    _, pos = tt.run_plan(ctx, tt.starts(sizes), parent, held, length, max_rows)
+    table = np.random.default_rng(3).permutation(len(sizes) * 60).reshape(-1, 60)
+    free, t = np.arange(3000) + 10 ** 6, {k: tt.i32(np.full(v, 77)) for k, v in dict(path=len(parent), count=len(sizes), next=len(sizes), length=len(sizes)).items()}
+    refused = np.array([m > max_rows for m in sizes])
+    want = tt.take_reference(sizes, parent, words, picks, held, np.where(refused, held, length))
+    back = [table[i, p] for i in range(len(sizes)) for p in range(-(-max(want["length"][i], 0) // page), -(-max(length[i], 0) // page))]
+    for at in (None, 3000):
+        got, kw = tt.i32(free), {}
+        if at:
+            kw = dict(table=tt.i32(table), page=page, free=got, taken=tt.i32([at]), taken_out=tt.i32([77]))
+        nunchi_amd.tree_take(ctx, *(tt.i32(x) for x in (tt.starts(sizes), parent, words, picks, held, length)), t["path"], t["count"], t["next"], t["length"],
+                             pos=tt.i32(pos), **kw)
+        assert all(np.array_equal(t[k].cpu().numpy(), want[k]) for k in t), [k for k in t if not np.array_equal(t[k].cpu().numpy(), want[k])]
+        if at:
+            assert kw["taken_out"].item() == at - len(back) and got[at - len(back):].tolist() == back
