@@ -434,7 +434,8 @@ int sh_tree_plan(sh_ctx* ctx, int n, int rows, const int32_t* cu, const int32_t*
 /* sh_page_attn for trees: the last cu[i + 1] - cu[i] of a request's len[i] positions are its rows' words. A row sees the shared
  * positions, its request's own before those words, and of the words those whose bits its mask has (its own bit set); its
  * position is that of the last own one before the words plus its bits, and the shape's window counts by it. A row without its
- * own bit, or of a request whose length is less than its rows, sees nothing: zeros and -inf. Masks need not come from sh_tree_plan: any bits of the request's words are followed.
+ * own bit, or of a request whose length is less than its rows, sees nothing: zeros and -inf. Masks need not come from
+ * sh_tree_plan: any bits of the request's words are followed, bits behind its rows count for nothing.
  * All else, work memory among it (sh_tree_attn_work), is as sh_page_attn says. max_rows 1 to 256; masks have
  * ceil(max_rows / 32) words a row. */
 int sh_tree_attn_work(const sh_page_shape* shape, int n, int rows, int max_rows, int prefix_len, int max_len, size_t* bytes);

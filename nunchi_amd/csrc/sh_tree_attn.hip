@@ -168,12 +168,14 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
         const bool node = held >= rows_k && nth >= 0 && nth < 32ll * a.words && (mask[nth >> 5] >> (nth & 31) & 1);
         int from = 0, first_word = 0;
         if (node && a.window) {
+            // (bits behind the request's rows are no words of its)
+            auto bits_of = [&](int w) { return mask[w] & (rows_k - 32 * w >= 32 ? ~0u : rows_k <= 32 * w ? 0u : (1u << (rows_k - 32 * w)) - 1); };
             int depth = -1;
-            for (int w = 0; w < a.words; w++) depth += __popc(mask[w]);
+            for (int w = 0; w < a.words; w++) depth += __popc(bits_of(w));
             from = (int)max(L0 + base + depth + 1ll - a.window, 0ll);
             int drop = depth + 1 - a.window;   // of the words that it follows the window leaves the last ones
             for (int w = 0; w < a.words && drop > 0; w++) {
-                unsigned bits = mask[w];
+                unsigned bits = bits_of(w);
                 const int n = __popc(bits);
                 if (n < drop) {
                     drop -= n;

@@ -103,3 +103,17 @@ def test_take_requests_that_the_plan_refused(ctx, page):
         assert all(np.array_equal(t[k].cpu().numpy(), want[k]) for k in t), [k for k in t if not np.array_equal(t[k].cpu().numpy(), want[k])]
         if at:
             assert kw["taken_out"].item() == at - len(back) and got[at - len(back):].tolist() == back
+
+
+@pytest.mark.parametrize("prefix,window", [(0, 0), (0, 3), (0, 40), (50, 7), (50, 64), (130, 100)])
+@pytest.mark.parametrize("D,kind", [(64, "f16"), (128, "bf16")])
+def test_attn_bits_behind_the_rows(ctx, D, kind, prefix, window):
+    """Bits of places that the request does not have move neither its rows' positions nor their windows."""
+    sizes, max_rows = [5, 40, 1, 32, 33, 64], 64
+    c = tt.tree_case(9, [30, 90, 8, 32, 70, 64], sizes, 8, 2, D, 16, kind, prefix=prefix, window=window, max_rows=max_rows)
+    mask, rng = c["mask"].cpu().numpy().view(np.uint64).reshape(-1).copy(), np.random.default_rng(2)
+    for r, m in enumerate(np.repeat(sizes, sizes)):
+        if m < 64:
+            mask[r] |= np.uint64(int(rng.integers(0, 2 ** 63)) >> m << m) | np.uint64(1 << 63)
+    c["mask"].copy_(torch.from_numpy(mask.view(np.int32).reshape(-1, 2)))
+    tt.check_tree(ctx, c)
