@@ -360,6 +360,8 @@ PyObject* tree_take(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (!table.none() && (!dims(table, "table", 2) || !fits(table, "table") || !has(table, "table", 2, n, table.d[1]) || !dims(free_pages, "free", 1) ||
                           !fits(free_pages, "free") || !has(taken, "taken", 1, 1) || !has(taken_out, "taken_out", 1, 1)))
         return nullptr;
+    // (a table of no columns has no address, but it is a table: what was taken is written)
+    if (!table.none() && !table.p) table.p = cu.p;
     return PyLong_FromLong(fn(ctx, (int)n, (int)rows, (const int32_t*)cu.p, (const int32_t*)parent.p, (const int32_t*)pos.p, (const int32_t*)words.p, (const int32_t*)picks.p,
                               (const int32_t*)held.p, (const int32_t*)length.p, (int32_t*)path.p, (int32_t*)count.p, (int32_t*)next.p, (int32_t*)length_out.p,
                               (int)page, (const int32_t*)table.p, (int)table.d[1], (int32_t*)free_pages.p, (int)free_pages.d[0], (const int32_t*)taken.p,

@@ -117,3 +117,12 @@ def test_attn_bits_behind_the_rows(ctx, D, kind, prefix, window):
             mask[r] |= np.uint64(int(rng.integers(0, 2 ** 63)) >> m << m) | np.uint64(1 << 63)
     c["mask"].copy_(torch.from_numpy(mask.view(np.int32).reshape(-1, 2)))
     tt.check_tree(ctx, c)
+
+
+@pytest.mark.parametrize("n", [2, 40])
+def test_take_of_a_table_without_columns(ctx, n):
+    """Nothing goes back, and what was taken is written all the same."""
+    sizes = [0] * n
+    for free, taken, left in (([], 0, 0), ([5, 6, 7], 2, 2), ([5, 6, 7], 9, 3), ([], 4, 0)):
+        got = tt.run_take(ctx, tt.starts(sizes), [], [], [], [3] * n, [3] * n, np.zeros((n, 0)), 16, np.array(free), taken)
+        assert got["taken"].tolist() == [left] and got["free"].tolist() == free and got["length"].tolist() == [3] * n
