@@ -426,8 +426,9 @@ int sh_sample(sh_ctx* ctx, int rows, int vocab, const void* scores, long long ld
  * and len). mask [rows][ceil(max_rows / 32)]: bit k of a row is set when the request's k-th row is the row itself or a word that
  * it follows; pos [rows]: pos0 + held + how many words it follows. A row whose parent, or a word that it follows, is not before
  * it, and all rows of a request that was refused (len is not held + its rows), that has more than max_rows rows or rows past
- * `rows`, get no bits and position -1: sh_page_put writes nothing for them and sh_tree_attn gives zeros. Rows behind the last
- * request's stay as they were. max_rows 1 to 256. */
+ * `rows`, get no bits and position -1. sh_page_put with a rotation table writes nothing for them (without one it goes by their
+ * slots alone, which no other row sees), sh_tree_attn gives zeros for them as far as they are among the first max_rows rows of their
+ * request (those past them stay as they were, below). Rows behind the last request's stay as they were. max_rows 1 to 256. */
 int sh_tree_plan(sh_ctx* ctx, int n, int rows, const int32_t* cu, const int32_t* parent, const int32_t* held, const int32_t* len,
                  int max_rows, uint32_t* mask, int32_t* pos, int pos0);
 
@@ -436,8 +437,8 @@ int sh_tree_plan(sh_ctx* ctx, int n, int rows, const int32_t* cu, const int32_t*
  * position is that of the last own one before the words plus its bits, and the shape's window counts by it. A row without its
  * own bit, or of a request whose length is less than its rows, sees nothing: zeros and -inf. Masks need not come from
  * sh_tree_plan: any bits of the request's words are followed, bits behind its rows count for nothing.
- * All else, work memory among it (sh_tree_attn_work), is as sh_page_attn says. max_rows 1 to 256; masks have
- * ceil(max_rows / 32) words a row. */
+ * Rows past max_rows of their request stay as they were. All else, work memory among it (sh_tree_attn_work), is as
+ * sh_page_attn says. max_rows 1 to 256; masks have ceil(max_rows / 32) words a row. */
 int sh_tree_attn_work(const sh_page_shape* shape, int n, int rows, int max_rows, int prefix_len, int max_len, size_t* bytes);
 int sh_tree_attn(sh_ctx* ctx, const sh_page_shape* shape, int n, int rows, const int32_t* cu, int max_rows, const uint32_t* mask,
                  const void* q, const void* keys, const void* values, const int32_t* prefix, int prefix_len,

@@ -126,3 +126,29 @@ def test_take_of_a_table_without_columns(ctx, n):
     for free, taken, left in (([], 0, 0), ([5, 6, 7], 2, 2), ([5, 6, 7], 9, 3), ([], 4, 0)):
         got = tt.run_take(ctx, tt.starts(sizes), [], [], [], [3] * n, [3] * n, np.zeros((n, 0)), 16, np.array(free), taken)
         assert got["taken"].tolist() == [left] and got["free"].tolist() == free and got["length"].tolist() == [3] * n
+
+
+@pytest.mark.parametrize("prefix", [0, 20, 7000])
+def test_rows_of_a_request_past_max_rows(ctx, prefix):
+    """Without bits: zeros and -inf for the first max_rows of them, whatever the keys, and the rows past these stay as they were. Writes
+    without a rotation table go by the slots; with one they pass such rows over."""
+    sizes, lens, max_rows = [3, 40, 2] + [1] * 16, [30, 90, 9] + [5] * 16, 32
+    parent = tt.trees(3, sizes)
+    sets = [None if 3 <= r < 43 else s for r, s in enumerate(tt.follows(parent, sizes))]
+    c = tt.tree_case(3, lens, sizes, 8, 2, 64, 16, "f16", prefix=prefix, gate=False, max_rows=max_rows, sets=sets)
+    mask, pos = tt.run_plan(ctx, tt.starts(sizes), parent, [a - b for a, b in zip(lens, sizes)], lens, max_rows)
+    assert (mask[3:43] == 0).all() and (pos[3:43] == -1).all()
+    assert np.array_equal(mask, c["mask"].cpu().numpy())
+    out, lse = tt.run_tree(ctx, c)
+    want, want_lse, tol, tol_lse = tt.tree_reference(c)
+    rows = [r for r in range(sum(sizes)) if not 35 <= r < 43]
+    assert ((out.cpu().double()[rows] - want[rows]).abs() <= tol[rows]).all() and (out[3:35] == 0).all() and (lse[3:35] == -float("inf")).all()
+    assert (out[35:43] == 7).all() and (lse[35:43] == 7).all()
+
+    shape = nunchi_amd.PageShape(1, 1, 32, 16, 4, dtype="f16")
+    qkv, slots, at = torch.ones(8, 96, device="cuda"), torch.arange(8).cuda() * 5, tt.i32([0, -1, 1, -1, -1, 2, 3, -1])
+    for rope in (None, torch.ones(5, 16, 2, device="cuda")):
+        keys, values = (torch.zeros(shape.cache_shape, dtype=torch.float16, device="cuda") for _ in range(2))
+        nunchi_amd.page_put(ctx, shape, qkv, slots, keys, values, pos=at, rope=rope)
+        there = (values.view(-1, 32)[slots] == 1).all(1)
+        assert there.tolist() == [rope is None or p >= 0 for p in at.tolist()]
