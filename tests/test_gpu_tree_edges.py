@@ -1,5 +1,7 @@
 """The operators for drafted words where plans, masks, pages and lengths are not the ordinary ones: what one of them refuses, the others do not
 take for whole. References and tolerances are tests/test_gpu_tree.py's."""
+import math
+
 import numpy as np
 import pytest
 
@@ -152,3 +154,25 @@ def test_rows_of_a_request_past_max_rows(ctx, prefix):
         nunchi_amd.page_put(ctx, shape, qkv, slots, keys, values, pos=at, rope=rope)
         there = (values.view(-1, 32)[slots] == 1).all(1)
         assert there.tolist() == [rope is None or p >= 0 for p in at.tolist()]
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_attn_many_small_weights(ctx, kind, D):
+    """20000 keys of weights 2^-25.5 of the largest, whose value is 0 and which the first block has: the output is the small ones' sum, as
+    close as page_attn's. Each weight is rounded by half a step (h, or 2^-25 below 2^-14 in f16: here 2^-25.52 + 11, the word's own 17.6875),
+    the result by h."""
+    N, n, page, h = 20000, 512, 16, tt.HALF[kind]
+    pages = N // page
+    keys, values = torch.zeros(pages, 2, page, D, dtype=tt.TYPES[kind], device="cuda"), torch.ones(pages, 2, page, D, dtype=tt.TYPES[kind], device="cuda")
+    q = torch.zeros(n, 2, D, dtype=tt.TYPES[kind], device="cuda")
+    q[..., 0] = 1
+    keys[0, :, 5, 0] = 17.6875
+    values[0, :, 5] = 0
+    shape = nunchi_amd.PageShape(2, 2, D, page, pages, dtype=kind, scale=1.0)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(n, 1)       # (all requests read the same pages)
+    out, work = torch.empty_like(q), torch.empty(nunchi_amd.tree_attn_work(shape, n, n, N, 1), dtype=torch.uint8, device="cuda")
+    nunchi_amd.tree_attn(ctx, shape, q, keys, values, table, tt.i32([N] * n), tt.i32(range(n + 1)), tt.i32([[1]] * n), out, work, N, 1)
+    e = math.exp(-keys[0, 0, 5, 0].item())
+    want = (N - 1) * e / (1 + (N - 1) * e)
+    assert ((out.double() / want - 1).abs() <= 2 * h + 2.0 ** -25 / 2.0 ** -14.52 + 2.0 ** -19).all(), out.double().mean().item() / want
