@@ -438,7 +438,8 @@ int sh_tree_plan(sh_ctx* ctx, int n, int rows, const int32_t* cu, const int32_t*
  * own bit, or of a request whose length is less than its rows, sees nothing: zeros and -inf. Masks need not come from
  * sh_tree_plan: any bits of the request's words are followed, bits behind its rows count for nothing.
  * Rows past max_rows of their request stay as they were. All else, work memory among it (sh_tree_attn_work), is as
- * sh_page_attn says. max_rows 1 to 256; masks have ceil(max_rows / 32) words a row. */
+ * sh_page_attn says. max_rows 1 to 256; masks have ceil(max_rows / 32) words a row. The same call gives the same bits; a row beside
+ * other rows, or in a batch of another size, may round elsewhere. */
 int sh_tree_attn_work(const sh_page_shape* shape, int n, int rows, int max_rows, int prefix_len, int max_len, size_t* bytes);
 int sh_tree_attn(sh_ctx* ctx, const sh_page_shape* shape, int n, int rows, const int32_t* cu, int max_rows, const uint32_t* mask,
                  const void* q, const void* keys, const void* values, const int32_t* prefix, int prefix_len,

@@ -102,7 +102,8 @@ __device__ __forceinline__ tile_of_request find_tile(const pattn_args& a, int at
 // their own.
 // Weights are rounded to the values' 16 bits for the second product; their sum stays in 32 bits. They are relative to a maximum
 // that is up to 2^SLACK behind the true one and 2^LIFT below it (sh_page_attn.hip says why). Each column is rescaled by its own
-// scores alone, so a row's result does not depend on the rows beside it.
+// scores alone, but its tile's other columns decide whether its first reference is four waves' or its own wave's, and under a window
+// which wave and part takes which key: the same call gives the same bits, a row beside other rows may round elsewhere.
 // SHARED: the columns of all requests over the shared positions. Else one request's columns over its own positions, and over the
 // shared ones before them where no SHARED part takes them (a.fused).
 template <class T, int D, int NT, bool SHARED>
