@@ -32,6 +32,14 @@ __device__ __forceinline__ int wave_isum(int v) {
     return v;
 }
 
+// what the wave's lanes wrote to LDS before is there for all of them behind it (one wave's LDS operations are done in order: no wait,
+// but nothing is moved across)
+__device__ __forceinline__ void wave_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Q4_0 block dot against an int8-cut input block. Codes are the 16 file bytes (byte i = column i in the low nibble,
 // column 16 + i in the high nibble); the input block is 8 dwords of int8 (columns 0..31). Codes 0..15 are valid
 // signed bytes, so the signed 4-way dot applies directly; the -8 offset is folded in by the caller.

@@ -265,16 +265,12 @@ __device__ __forceinline__ void attend(const pattn_args& a, const int block, tre
         auto turn_keys = [&]() {
 #pragma unroll
             for (int n = 0; n < KI; n++) *(u32x4*)(kw + n * RI * (D + 8)) = kr[n];
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            wave_lds();
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int c = 0; c < CH; c++) kf[h][c] = *(const u32x4*)(ks + h * 16 * (D + 8) + c * 32);
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            wave_lds();
         };
         auto load_values = [&](unsigned half0, unsigned half1) {
 #pragma unroll
