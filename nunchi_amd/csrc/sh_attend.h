@@ -1,5 +1,5 @@
-// What the attention kernels over pages share (sh_page_attn.hip, sh_tree_attn.hip): the matrix instructions of either type,
-// the rounding and rescaling of weights, and the space in which the four waves of a workgroup are joined.
+// What the attention kernels over pages share (sh_page_attn.hip, sh_tree_attn.hip): the matrix instructions of either type, the
+// rounding and rescaling of weights, and the request of a row.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -33,18 +33,10 @@ template <class T> __device__ __forceinline__ unsigned pack2(float x, float y) {
     const t2 v = {(T)x, (T)y};   // to nearest
     return __builtin_bit_cast(unsigned, v);
 }
-template <class T> __device__ __forceinline__ float of_bits(unsigned h) {
-    return (float)__builtin_bit_cast(T, (unsigned short)h);
-}
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 // e^(from - to) in powers of two for maxima that may be -inf (nothing seen yet)
 __device__ __forceinline__ float rescale(float from, float to) { return from == -INFINITY ? 0.0f : exp2_(from - to); }
 
-template <class F> __device__ __forceinline__ int over16(int v, F f) {   // the same value in the 16 lanes of a column group
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) v = f(v, __shfl_xor(v, o));
-    return v;
-}
 // the request whose rows hold `row` (the last k with cu[k] <= row)
 __device__ __forceinline__ int request_of(const int32_t* cu, int n, int row) {
     int x = 0, y = n;
@@ -55,19 +47,6 @@ __device__ __forceinline__ int request_of(const int32_t* cu, int n, int row) {
     }
     return x;
 }
-
-// what the four waves of a workgroup pass each other when they are joined: 16 NT columns of D sums (the pitch shifts
-// columns by four banks), maxima and sums of weights, of two waves
-template <int D, int NT> struct join_space {
-    static constexpr int NC = 16 * NT, PITCH = D + 4;
-    float o[2][NC * PITCH];
-    float m[2][NC], l[2][NC];
-};
-
-// column groups of 16 a workgroup takes: one, or as many as the registers hold (prompts of 300 rows, head_dim 128: 40 us
-// in tiles of 32 columns, 84 in tiles of 16, which read every key twice as often)
-constexpr int attn_many(int D) { return D > 64 ? 2 : 4; }
-inline int attn_col_groups(int D, long long cols) { return cols <= 16 ? 1 : attn_many(D); }
 
 }  // namespace
 }  // namespace sh

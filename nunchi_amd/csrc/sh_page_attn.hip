@@ -15,6 +15,25 @@
 
 namespace sh {
 namespace {
+
+template <class T> __device__ __forceinline__ float of_bits(unsigned h) {
+    return (float)__builtin_bit_cast(T, (unsigned short)h);
+}
+
+template <class F> __device__ __forceinline__ int over16(int v, F f) {   // the same value in the 16 lanes of a column group
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v = f(v, __shfl_xor(v, o));
+    return v;
+}
+
+// what the four waves of a workgroup pass each other when they are joined: 16 NT columns of D sums (the pitch shifts
+// columns by four banks), maxima and sums of weights, of two waves
+template <int D, int NT> struct join_space {
+    static constexpr int NC = 16 * NT, PITCH = D + 4;
+    float o[2][NC * PITCH];
+    float m[2][NC], l[2][NC];
+};
+
 // Keys are counted along one line: the shared positions, a gap to the next multiple of 32, the request's own.
 // Columns: the (row, query head) pairs of one kv head, packed; a workgroup takes 16 NT of them and one part of the line,
 // its four waves take blocks of 32 keys in turn. With K of 32 keys as rows of the first product (S^T = K Q^T) a lane
@@ -418,6 +437,11 @@ __global__ __launch_bounds__(256) void k_page_join(pattn_args a) {
     if (a.lse && d == 0) a.lse[rh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
+// column groups of 16 a workgroup takes: one, or as many as the registers hold (prompts of 300 rows, head_dim 128: 40 us
+// in tiles of 32 columns, 84 in tiles of 16, which read every key twice as often)
+constexpr int many(int D) { return D > 64 ? 2 : 4; }
+int col_groups(int D, long long cols) { return cols <= 16 ? 1 : many(D); }
+
 long long shared_tiles(const pattn_args& a, int nt) { return ((long long)a.rows * a.grp + 16 * nt - 1) / (16 * nt); }
 long long own_tiles(const pattn_args& a, int nt, bool single) {
     return single ? (long long)a.n * ((a.grp + 16 * nt - 1) / (16 * nt)) : (long long)a.rows * a.grp / (16 * nt) + a.n;
@@ -436,8 +460,8 @@ template <class T, int D> hipError_t run_join(const pattn_args& a, hipStream_t s
     return hipGetLastError();
 }
 template <class T, int D> hipError_t run_all(const pattn_args& a, hipStream_t s) {
-    constexpr int M = attn_many(D);
-    const int nts = a.sp ? attn_col_groups(D, (long long)a.rows * a.grp) : 0, nto = attn_col_groups(D, (long long)a.max_rows * a.grp);
+    constexpr int M = many(D);
+    const int nts = a.sp ? col_groups(D, (long long)a.rows * a.grp) : 0, nto = col_groups(D, (long long)a.max_rows * a.grp);
     hipError_t e;
     if (nts == 0) e = nto == 1 ? run_attn<T, D, 0, 1>(a, s) : run_attn<T, D, 0, M>(a, s);
     else if (nts == 1) e = run_attn<T, D, 1, 1>(a, s);   // (a request has no more columns than all of them)
@@ -464,8 +488,8 @@ void split(long long base, long long range, long long want, int* parts, int* chu
 // unit (two for the shared positions), of 256 keys or more. With twice as many parts 48 requests of 4096 positions took 63 to
 // 66 us instead of 62, the prompts below 76 instead of 40.
 bool page_attn_split(int D, bool single, pattn_args& a) {
-    const int nto = attn_col_groups(D, (long long)a.max_rows * a.grp);
-    const long long own = own_tiles(a, nto, single), all = shared_tiles(a, attn_col_groups(D, (long long)a.rows * a.grp));
+    const int nto = col_groups(D, (long long)a.max_rows * a.grp);
+    const long long own = own_tiles(a, nto, single), all = shared_tiles(a, col_groups(D, (long long)a.rows * a.grp));
     a.own_at = (a.prefix_len + 31) / 32 * 32;
     // Requests whose columns fill their workgroups read the shared positions themselves: sharing would not save reads,
     // and nothing has to be joined (13 prompts of 300 rows behind 500 positions: 40 us, 138 apart). us fused and apart for 16

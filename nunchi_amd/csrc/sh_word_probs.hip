@@ -65,7 +65,6 @@ template <class V> __device__ __forceinline__ V wave_all(V v, V (*f)(V, V)) {
 __device__ __forceinline__ int add_i(int x, int y) { return x + y; }
 __device__ __forceinline__ float add_f(float x, float y) { return x + y; }
 __device__ __forceinline__ float most_f(float x, float y) { return fmaxf(x, y); }
-__device__ __forceinline__ unsigned most_u(unsigned x, unsigned y) { return max(x, y); }
 
 // A number that at least n of the wave's keys (N a lane) reach, and at most a few more than n: the n-th largest bit by bit, until
 // that is so.
