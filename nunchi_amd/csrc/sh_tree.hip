@@ -2,7 +2,7 @@
 // and the pages that are free again after it (k_tree_free), and the branch's keys and values at their places (k_page_keep).
 //
 // All are bound by latency: 256 requests of 64 words read and write 1 MB (plan), 0.3 MB (take), 16 MB (keep, of up to 15 moved
-// words); a kernel with its dependent loads takes 2.5 to 6 us, and the calling thread 8 to 10 us for each call that it makes.
+// words); a kernel with its dependent loads takes 2.6 to 6.4 us, and the calling thread 8 to 10 us for each call that it makes.
 #include <hip/hip_runtime.h>
 
 #include <climits>

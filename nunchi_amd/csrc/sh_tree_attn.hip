@@ -5,11 +5,12 @@
 // With a column's reference r, its sum l of e^(s - r) and its sums O of e^(s - r) v over the keys that it sees, two waves or parts have
 // r' = max(r1, r2), l' = l1 e^(r1 - r') + l2 e^(r2 - r'), O' likewise, and the result is O / l (0 where nothing is seen).
 //
-// What bounds it: many columns, issue: 64 requests of up to 64 words over 2048 shared and 2048 own positions (8 kv heads of 64, 56
-// GFLOP) 120 to 133 us, 420 to 470 TFLOP/s of 1139, of which the exponentials, conversions and masks take as long as the products,
-// and 2.1 rounds of workgroups over the compute units; few columns over long keys, memory: 64 requests x 4 words behind 2048 shared
-// and 2048 own positions 35 us, 4.8 TB/s of 5.0; one request, the chain of loads in front of the first product (ids, keys, 5 us) and
-// the join of its parts (6 us of 22 to 29 for 32749 positions); short ones, the launch.
+// What bounds it (us a call, calls in a row over three inputs in turn): many columns, issue: 64 requests of up to 64 words over 2048
+// shared and up to 2048 own positions (8 kv heads of 64, 54 GFLOP) 124 us, 440 TFLOP/s of 1139, of which the exponentials, conversions
+// and masks take as long as the products, and 2.1 rounds of workgroups over the compute units; few columns over long keys, memory: 64
+// requests x 4 words over the same positions (156 MB) 46.5, 3.4 TB/s of 5.0, and 35.7 where the same input comes again and the last
+// cache still has it; one request, the chain of loads in front of the first product (ids, keys, 5 us) and the join of its parts (6 us
+// of 27 for 32749 positions); short ones, the launch.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -663,10 +664,14 @@ bool tree_attn_split(int D, pattn_args& a) {
     // Column groups of 16 a workgroup takes. Wide tiles read a block of keys fewer times, narrow ones make more workgroups that run
     // at once, so the work of all columns decides (columns times positions times kv heads, w; heads of 128 twice), where one group does
     // not hold a request's columns. us by 1, 2 and 4 groups of heads of 64, 8 kv heads: 64 requests x 8 words over 500 positions (w 4
-    // million) 12.9, 16.5 and 28.9, one of 64 words over 4096 (8) 15.8, 18.2 and 23.2, 8 x 64 over 2500 (23) 23.2, 21.5 and 33.9; 64 x
-    // 32 over 4096 (136) 118, 86 and 92, 64 x 64 over 4096 (273) 222, 147 and 138. Four groups of heads of 128 do not fit the registers;
-    // by 1 and 2, 4 kv heads: one of 64 words over 4096 (8) 15.0 and 18.2, one of 32 over 16000 (16) 17.0 and 20.1, 64 x 16 over 500
-    // (8) 22.9 and 21.7, 8 x 64 over 2500 (23) 26.8 and 23.9, 64 x 64 over 4096 (273) 186 and 134
+    // million) 13.0, 14.5 and 22.4, 64 x 16 over 500 (8) 18.0, 18.7 and 23.8, one of 64 words over 4096 (8) 14.6, 14.1 and 17.3, one of 32
+    // over 16000 (16) 19.4, 17.6 and 20.3, 8 x 64 over 2500 (23) 21.5, 20.4 and 24.6, one of 256 over 4096 (34) 23.8, 20.3 and 28.7, 64 x
+    // 32 over 4096 (136) 120, 94.8 and 89.0, 64 x 64 over 4096 (273) 176, 127 and 113. Four groups of heads of 128 do not fit the
+    // registers; by 1 and 2, 4 kv heads: one of 64 words over 4096 (8) 14.6 and 18.5, 64 x 16 over 500 (8) 21.7 and 20.2, one of 32 over
+    // 16000 (16) 19.5 and 21.1, 8 x 64 over 2500 (23) 24.4 and 23.0, one of 256 over 4096 (34) 21.3 and 24.8, one of 33 over 32749 (35)
+    // 30.6 and 27.2, 64 x 64 over 4096 (273) 180 and 143. Work alone does not tell a long request from a batch: the rule takes the slower
+    // side for 64 x 32 over 4096 (by 7 %) and, in heads of 128, for 64 x 16 over 500 (7), one of 32 over 16000 (8) and one of 256 over
+    // 4096 (16)
     a.nts = cols <= 16 ? 1 : 2;
     auto groups = [&](long long range) {
         if (a.window) range = std::min(range, a.window + 63ll + a.max_rows);
@@ -700,7 +705,7 @@ bool tree_attn_split(int D, pattn_args& a) {
     // One workgroup per compute unit, of 512 keys or more: one request of 64 words over 33000 positions (8 kv heads of 64) 32 us, with
     // three quarters as many parts 37, with one and a half times as many 35 (the join reads all of them); 4 kv heads of 128 31, 34 and 36.
     // 64 requests x 4 words behind 2048 shared positions, 4 kv heads of 128, by 256, 512 and 1024 keys a part 44.8, 39.7 and 38.5,
-    // 8 of 64 35.4, 35.1 and 38.6
+    // 8 of 64 35.4, 35.1 and 38.6 (one input again and again)
     split(std::max((cols + 16 * a.nto - 1) / (16 * a.nto), (long long)a.n), range, 256, &a.so, &a.ochunk);
     const long long shared_blocks = all * a.n_kv * a.sp, own_blocks = own * a.n_kv * a.so;
     const long long rh = (long long)a.rows * a.n_head, join = a.sp + a.so == 1 ? 0 : a.sp + a.so > 16 ? rh : (rh + 3) / 4;

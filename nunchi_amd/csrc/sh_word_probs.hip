@@ -10,8 +10,9 @@
 // it. No histogram, no sort. A word's place in the order is one 64-bit key: its score as a number that sorts like it, and its
 // index turned round.
 //
-// What bounds it: many rows, memory (256 rows of 97496 fp32 scores, 100 MB: 21 to 23 us for the parts, 4.3 to 4.8 TB/s of 5.0, and 4.9
-// for the join); few rows, the two launches that wait for each other (one such row 6.0 and 3.5 us of kernels, 12 a call).
+// What bounds it: many rows, memory (256 rows of 97496 fp32 scores, 100 MB: 23.3 us for the parts, 4.3 TB/s of 5.0, and 4.8 for the join; a
+// call 27.2. In 16 bits, 50 MB, a call takes 25: as many words, each with its exponential); few rows, the two launches that wait for each
+// other (one such row 6.0 and 3.5 us of kernels, 11.4 a call).
 #include <hip/hip_runtime.h>
 
 #include <climits>
