@@ -468,11 +468,11 @@ int sh_word_probs(sh_ctx* ctx, int rows, int vocab, const void* scores, long lon
  *   next    [n]     the pick after the last kept row: the word that the next step starts with (-1 where there is none)
  *   len_out [n]     held + count
  * Picks below 0 agree with nothing. A request without rows keeps its length; one whose length is not held + its rows, or that has
- * more than 256 rows, keeps nothing, its len_out is len. One whose first row has a parent that is not -1 keeps nothing either,
- * its len_out is held: none of its rows were written. With table [n][cols] (null: not done) the pages between ceil(len_out /
- * page) and ceil(len / page) of each request go back, in the order of the requests: *taken of free_pages [n_free] were given out
- * (sh_page_plan's taken_out), *taken_out is that less the pages that go back, which are written from free_pages[*taken_out] on;
- * pages past *taken are not written. n up to 4096. */
+ * more than 256 rows, keeps nothing, its len_out is len (held with sh_tree_take_planned, for a request that has more rows than
+ * its tree may). One whose first row has a parent that is not -1 keeps nothing either, its len_out is held: none of its rows were
+ * written. With table [n][cols] (null: not done) the pages between ceil(len_out / page) and ceil(len / page) of each request go
+ * back, in the order of the requests: *taken of free_pages [n_free] were given out (sh_page_plan's taken_out), *taken_out is that
+ * less the pages that go back, which are written from free_pages[*taken_out] on; pages past *taken are not written. n up to 4096. */
 int sh_tree_take(sh_ctx* ctx, int n, int rows, const int32_t* cu, const int32_t* parent, const int32_t* words,
                  const int32_t* picks, const int32_t* held, const int32_t* len, int32_t* path, int32_t* count, int32_t* next,
                  int32_t* len_out, int page, const int32_t* table, int cols, int32_t* free_pages, int n_free,
