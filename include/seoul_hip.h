@@ -478,9 +478,10 @@ int sh_tree_take(sh_ctx* ctx, int n, int rows, const int32_t* cu, const int32_t*
                  int32_t* len_out, int page, const int32_t* table, int cols, int32_t* free_pages, int n_free,
                  const int32_t* taken, int32_t* taken_out);
 
-/* The same for a step whose plan may have refused requests that sh_page_plan took, as one of more than its max_rows rows: pos
- * [rows] are sh_tree_plan's positions (null: sh_tree_take). A request whose first row has none (below 0) keeps nothing and its
- * len_out is held, whatever its number of rows, so that no position counts that was not written. */
+/* The same for a step whose plan may have refused requests that sh_page_plan took, as one of more than its max_rows rows, which
+ * sh_tree_take cannot tell from the others (it knows no max_rows): pos [rows] are sh_tree_plan's positions (null: sh_tree_take).
+ * A request whose first row has none (below 0) keeps nothing and its len_out is held, whatever its number of rows, so that no
+ * position counts that was not written. */
 int sh_tree_take_planned(sh_ctx* ctx, int n, int rows, const int32_t* cu, const int32_t* parent, const int32_t* pos,
                          const int32_t* words, const int32_t* picks, const int32_t* held, const int32_t* len, int32_t* path,
                          int32_t* count, int32_t* next, int32_t* len_out, int page, const int32_t* table, int cols,

@@ -154,7 +154,8 @@ def tree_take(ctx, cu, parent, words, picks, held, length, path, count, next, le
     """The branch of drafted words that the picks agree with (sh_tree_take): cu [n + 1], parent, words and picks [rows], held
     and length [n] i32 in; path [rows], count, next and length_out [n] i32 out. With table [n][cols] i32 the pages behind the
     new lengths go back to free [n_free] i32, taken [1] i32 in and taken_out [1] out. With pos [rows] i32, tree_plan's, requests
-    that it refused keep nothing and the length they had (sh_tree_take_planned)."""
+    that it refused keep nothing and the length they had (sh_tree_take_planned); without it a request of more rows than the
+    plan's max_rows counts as planned."""
     native = _native or _load()
     rc = native[0].tree_take(native[8], ctx.h.value, ctx.device, cu, parent, words, picks, held, length, path, count, next, length_out, table, page, free,
                              taken, taken_out, pos)
